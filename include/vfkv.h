@@ -465,6 +465,154 @@ int vfkv_prefill_attention_gated(vfkv_cache* c, uint32_t layer, uint32_t kv_laye
                                  const float* q, float* o, uint32_t m, uint32_t base_pos, uint32_t window,
                                  float scale, float softcap, const vfkv_gate* gate, vfkv_stream stream);
 
+/* ------------------------------------------------------------------------------------------ */
+/* Paged cache: several sequences of different lengths over one pool of pages.                */
+/* ------------------------------------------------------------------------------------------ */
+/* No counterpart in the reference, whose cache holds one sequence (kv_cache.rs:204-223).  K and V are
+ * [layer][page][kv_head][slot][d] in the cache dtype: a page holds `page_size` consecutive positions of one
+ * sequence in every layer, and one KV head's rows of a page are contiguous (what an attention workgroup
+ * reads).  Position j of a sequence lives in slot j % page_size of page page_table[j / page_size].
+ * The object also counts the references of every page on the host (alloc, retain, release, fork, compact);
+ * the compute entry points only look at the device page tables, so callers with a page manager of their own
+ * may ignore the counts. */
+typedef struct vfkv_pages_config {
+    uint32_t n_layers;
+    uint32_t n_kv_heads;
+    uint32_t head_dim;  /* <= 512; multiples of 16 up to 256 run on the matrix cores */
+    uint32_t page_size; /* positions per page: 16, 32, 64, 128 or 256 */
+    uint32_t n_pages;   /* n_pages * page_size <= 2^31 - 1 */
+    uint32_t dtype;     /* vfkv_dtype */
+} vfkv_pages_config;
+
+typedef struct vfkv_pages vfkv_pages;
+#define VFKV_NO_PAGE 0xFFFFFFFFu /* page table entry without a page (-1 in the int32 device tables) */
+
+/* Device allocations (not cleared) on the current device. */
+int vfkv_pages_create(const vfkv_pages_config* cfg, vfkv_pages** out);
+/* The same over caller-owned buffers of vfkv_pages_bytes_per_buffer bytes, 16-byte aligned, on the current device (both
+ * NULL: layout and page counting only). */
+int vfkv_pages_create_external(const vfkv_pages_config* cfg, void* k_buffer, void* v_buffer, vfkv_pages** out);
+void vfkv_pages_destroy(vfkv_pages* c);
+void* vfkv_pages_k_ptr(const vfkv_pages* c);
+void* vfkv_pages_v_ptr(const vfkv_pages* c);
+uint64_t vfkv_pages_bytes_per_buffer(const vfkv_pages* c);
+uint64_t vfkv_pages_offset_bytes(const vfkv_pages* c, uint32_t layer, uint32_t page); /* start of a page in either buffer */
+
+/* Page counting (host only, immediate).  Calls on one object must not overlap in time. */
+uint32_t vfkv_pages_free_count(const vfkv_pages* c);
+uint32_t vfkv_pages_refcount(const vfkv_pages* c, uint32_t page); /* 0 = free (or out of range) */
+/* The n lowest free pages, in ascending order, one reference each.  VFKV_ERR_WORKSPACE when fewer are free; nothing is
+ * taken then. */
+int vfkv_pages_alloc(vfkv_pages* c, uint32_t n, uint32_t* pages_out);
+/* One more / one less reference per entry (VFKV_NO_PAGE entries are skipped); a page is free again at zero.  An
+ * entry that is out of range or free (counting the entry's repetitions in this call) is an error and changes nothing.
+ * A released page may be handed out again at once: work already enqueued that reads it must be ahead of the work that
+ * overwrites it in stream order. */
+int vfkv_pages_retain(vfkv_pages* c, const uint32_t* pages, uint32_t n);
+int vfkv_pages_release(vfkv_pages* c, const uint32_t* pages, uint32_t n);
+
+/* Copies the first rows[i] slots (rows NULL: all page_size) of page src[i] to page dst[i], all layers and heads, K and V, for
+ * i < n.  src, dst and rows are HOST arrays, read before the call returns (a captured call replays the same copies).
+ * Destinations must be distinct and none may be a source of the same call (VFKV_ERR_INVALID_ARG); reference counts
+ * are neither checked nor changed. */
+int vfkv_pages_copy(vfkv_pages* c, const uint32_t* src, const uint32_t* dst, const uint32_t* rows, uint32_t n,
+                    vfkv_stream stream);
+/* n_forks continuations of a sequence of kv_len positions whose ceil(kv_len / page_size) pages are `pages` (all live; entries
+ * behind a sliding window may be VFKV_NO_PAGE and stay so): pages_out [n_forks][same count] shares the full pages (one
+ * reference each) and gives each fork a page of its own for a last page that is not full, with the rows copied.
+ * VFKV_ERR_WORKSPACE when the free pages do not suffice; nothing changes then. */
+int vfkv_pages_fork(vfkv_pages* c, const uint32_t* pages, uint32_t kv_len, uint32_t n_forks, uint32_t* pages_out,
+                    vfkv_stream stream);
+/* Moves the live pages into the lowest ids: live pages with an id at or above the number of live pages are copied into the free
+ * ids below it, both taken in ascending order.  new_ids_out [n_pages] receives every live page's new id (unmoved pages
+ * keep theirs) and VFKV_NO_PAGE for free ones; the caller rewrites its page tables with it. */
+int vfkv_pages_compact(vfkv_pages* c, uint32_t* new_ids_out, vfkv_stream stream);
+
+/* A batch of sequences.  The three arrays are DEVICE arrays, read when the work runs, so a captured call follows them from replay
+ * to replay.  Sequence s owns the token rows [q_offsets[s], q_offsets[s + 1]) of q / k / v / o (q_offsets NULL:
+ * n_tokens == n_seqs, row s); they are its last positions: row i of m has position kv_lens[s] - m + i, and
+ * kv_lens[s] counts them.  Values the kernels cannot use are bounded, never followed: kv_lens are clamped to
+ * [0, table_stride * page_size], q_offsets to [0, n_tokens]; a page table entry outside [0, n_pages) has no rows (writes to it
+ * are dropped, its keys are invisible), a token at a negative position has neither row nor visible keys.
+ * Rows of no sequence (n_tokens may exceed q_offsets[n_seqs]) are left as they were. */
+typedef struct vfkv_seq_batch {
+    const int32_t* page_table; /* [n_seqs][table_stride] */
+    const int32_t* kv_lens;    /* [n_seqs] */
+    const int32_t* q_offsets;  /* [n_seqs + 1], not decreasing, or NULL: one token per sequence */
+    uint32_t n_seqs;           /* <= 8192 */
+    uint32_t table_stride;     /* page table entries per sequence */
+    uint32_t n_tokens;         /* rows of q / k / v / o */
+    uint32_t max_kv_len;       /* upper bound of kv_lens that sizes the launch (0: none known).  Results do not depend on it. */
+} vfkv_seq_batch;
+
+/* Norm, rotation and append of a batch: what vfkv_qk_rope_kv_write does for one sequence (executor/attention.rs:360-597), with
+ * positions of several axes (the time / height / width positions of image and video tokens; GGML_ROPE_TYPE_MROPE,
+ * which the reference's rope shaders leave out).  Pair p of a row turns by
+ *     positions[axis(p)][token] * freq_base^(-2 p / rotary_dim) / freq_factors[p] * freq_scale
+ * computed in 64 bits up to the reduction to one turn: far positions lose nothing.  section[a] counts the pairs of axis a and
+ * the sections add up to rotary_dim / 2.  interleaved == 0: axis 0 has the first section[0] pairs, axis 1 the next ones and
+ * so on.  interleaved == 1: pair p has axis p % n_axes while p / n_axes < section[p % n_axes], and axis 0 otherwise. */
+typedef struct vfkv_mrope_params {
+    uint32_t rope_mode;   /* VFKV_ROPE_NORM / VFKV_ROPE_NEOX */
+    uint32_t rotary_dim;  /* even, <= head_dim; 0: no rotation */
+    uint32_t n_axes;      /* 1..4 */
+    uint32_t interleaved;
+    uint32_t section[4];  /* ignored with one axis */
+    float freq_base;      /* > 0 */
+    float freq_scale;     /* finite; 1.0 usually */
+    float attn_factor;    /* 1.0 usually */
+    float eps;            /* of the RMS norm */
+} vfkv_mrope_params;
+
+/* q [n_tokens][n_heads][head_dim] (NULL: no query rows) is normalised (q_norm_weight [head_dim] f32, NULL: no norm) and rotated
+ * into q_out (which may be q); k and v [n_tokens][n_kv_heads][head_dim] are appended at their tokens' positions, k
+ * normalised and rotated first.  io_dtype (VFKV_F32 / VFKV_F16) is the type of q, k, v and q_out; *_stride the elements between two
+ * tokens' rows (0: contiguous), so slices of one projection output need no copy.  positions [n_axes][n_tokens] int32 on the
+ * device, NULL: every axis has the token's position in its sequence (one per token: n_axes rows of them otherwise).
+ * freq_factors [rotary_dim / 2] f32 on the device or NULL.  Two sequences that share a page must not both append to it. */
+typedef struct vfkv_paged_rows {
+    const void* q;
+    const float* q_norm_weight;
+    void* q_out;
+    const void* k;
+    const void* v;
+    const float* k_norm_weight;
+    const int32_t* positions;
+    const float* freq_factors;
+    uint32_t n_heads;
+    uint32_t io_dtype;
+    uint32_t q_stride, q_out_stride, k_stride, v_stride;
+} vfkv_paged_rows;
+int vfkv_paged_qk_rope_kv_write(vfkv_pages* c, uint32_t layer, const vfkv_seq_batch* b, const vfkv_paged_rows* rows,
+                                const vfkv_mrope_params* p, vfkv_stream stream);
+
+/* What a query sees and how its scores are formed.  The query at position p sees key j when j <= p and
+ * (window == 0 or j > p - window or j < n_sink): a sliding window behind a few first tokens that stay visible.  A query
+ * that sees nothing gets zeros. */
+typedef struct vfkv_paged_attn_params {
+    uint32_t n_heads;
+    uint32_t window;   /* 0: all keys up to the query's own */
+    uint32_t n_sink;
+    uint32_t io_dtype; /* VFKV_F32 / VFKV_F16: type of q and o */
+    uint32_t q_stride; /* elements between two tokens' rows; 0: n_heads * head_dim */
+    uint32_t o_stride;
+    float scale;       /* positive, finite */
+    float softcap;     /* as in vfkv_decode_attention; 0: none */
+} vfkv_paged_attn_params;
+
+/* Scratch of the two attention calls for one cache geometry; independent of the number and length of the sequences.  Calls that
+ * share a workspace must be ordered on one stream (two captured graphs that share one must not run at the same time). */
+int vfkv_paged_workspace_create(const vfkv_pages* c, uint32_t n_heads, vfkv_workspace** out);
+
+/* One token per sequence (b->q_offsets NULL, n_tokens == n_seqs): q, o [n_seqs][n_heads][head_dim].  The keys of the whole batch
+ * are dealt evenly to the workgroups, whatever the lengths; parts of a sequence are joined by log-sum-exp. */
+int vfkv_paged_decode_attention(vfkv_pages* c, uint32_t layer, const vfkv_seq_batch* b, const vfkv_paged_attn_params* p,
+                                const void* q, void* o, vfkv_workspace* ws, vfkv_stream stream);
+/* Any number of tokens per sequence, causal: chunks of prompts, drafted tokens, decode tokens among them.  ws may be NULL:
+ * short chunks over long contexts then run without a split over the keys. */
+int vfkv_paged_prefill_attention(vfkv_pages* c, uint32_t layer, const vfkv_seq_batch* b, const vfkv_paged_attn_params* p,
+                                 const void* q, void* o, vfkv_workspace* ws, vfkv_stream stream);
+
 #if defined(__GNUC__) || defined(__clang__)
 #pragma GCC visibility pop
 #endif

@@ -11,6 +11,9 @@ from ._ffi import VfkvError, lib, lib_path  # noqa: F401
 from .kv_cache import (KvCache, KvCacheConfig, KvDtype, guard_kv_precision, kv_bytes_per_token,  # noqa: F401
                        gemma4_kv_read_layer, build_kv_sources, prefix_reuse_start)
 from .forward import Forward, Workspace  # noqa: F401
+from .paged import MRope, PagedForward, PagedKvCache, PagedKvConfig, PagedWorkspace, SeqBatch  # noqa: F401
+from ._ffi import ROPE_NEOX, ROPE_NORM  # noqa: F401
 
 __all__ = ["KvCache", "KvCacheConfig", "KvDtype", "Forward", "Workspace", "VfkvError", "lib", "lib_path",
-           "guard_kv_precision", "kv_bytes_per_token", "gemma4_kv_read_layer", "build_kv_sources", "prefix_reuse_start"]
+           "guard_kv_precision", "kv_bytes_per_token", "gemma4_kv_read_layer", "build_kv_sources", "prefix_reuse_start",
+           "PagedKvCache", "PagedKvConfig", "PagedForward", "PagedWorkspace", "SeqBatch", "MRope", "ROPE_NORM", "ROPE_NEOX"]

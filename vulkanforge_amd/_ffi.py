@@ -46,6 +46,35 @@ class Gate(C.Structure):
     _fields_ = [("gate", C.c_void_p), ("chunk", C.c_uint32), ("stride", C.c_uint32), ("gate_offset", C.c_uint32)]
 
 
+class PagesConfig(C.Structure):
+    _fields_ = [("n_layers", C.c_uint32), ("n_kv_heads", C.c_uint32), ("head_dim", C.c_uint32),
+                ("page_size", C.c_uint32), ("n_pages", C.c_uint32), ("dtype", C.c_uint32)]
+
+
+class SeqBatchArgs(C.Structure):
+    _fields_ = [("page_table", C.c_void_p), ("kv_lens", C.c_void_p), ("q_offsets", C.c_void_p), ("n_seqs", C.c_uint32),
+                ("table_stride", C.c_uint32), ("n_tokens", C.c_uint32), ("max_kv_len", C.c_uint32)]
+
+
+class MRopeParams(C.Structure):
+    _fields_ = [("rope_mode", C.c_uint32), ("rotary_dim", C.c_uint32), ("n_axes", C.c_uint32), ("interleaved", C.c_uint32),
+                ("section", C.c_uint32 * 4), ("freq_base", C.c_float), ("freq_scale", C.c_float),
+                ("attn_factor", C.c_float), ("eps", C.c_float)]
+
+
+class PagedRows(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("q_norm_weight", C.c_void_p), ("q_out", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("k_norm_weight", C.c_void_p), ("positions", C.c_void_p), ("freq_factors", C.c_void_p),
+                ("n_heads", C.c_uint32), ("io_dtype", C.c_uint32), ("q_stride", C.c_uint32), ("q_out_stride", C.c_uint32),
+                ("k_stride", C.c_uint32), ("v_stride", C.c_uint32)]
+
+
+class PagedAttnParams(C.Structure):
+    _fields_ = [("n_heads", C.c_uint32), ("window", C.c_uint32), ("n_sink", C.c_uint32), ("io_dtype", C.c_uint32),
+                ("q_stride", C.c_uint32), ("o_stride", C.c_uint32), ("scale", C.c_float), ("softcap", C.c_float)]
+
+
+NO_PAGE = 0xFFFFFFFF   # VFKV_NO_PAGE
 PREFILL_F16_WEIGHTS, PREFILL_FP8_SCORES, PREFILL_F16_QUERIES = 1, 2, 4   # the VFKV_PREFILL_* option bits
 ROPE_NORM, ROPE_NEOX = 0, 2   # GGML_ROPE_TYPE_NORMAL / _NEOX (rms_norm.comp:25-26)
 
@@ -112,6 +141,25 @@ SIGNATURES = {
     "vfkv_prefill_attention_opt": (C.c_int, [_vp, _u32, _u32, _u32, _vp, _vp, _u32, _u32, _u32, _f, _f, _u32, _vp, _vp]),
     "vfkv_prefill_attention": (C.c_int, [_vp, _u32, _u32, _u32, _vp, _vp, _u32, _u32, _u32, _f, _f, _vp]),
     "vfkv_prefill_attention_ws": (C.c_int, [_vp, _u32, _u32, _u32, _vp, _vp, _u32, _u32, _u32, _f, _f, _vp, _vp]),
+    "vfkv_pages_create": (C.c_int, [C.POINTER(PagesConfig), C.POINTER(_vp)]),
+    "vfkv_pages_create_external": (C.c_int, [C.POINTER(PagesConfig), _vp, _vp, C.POINTER(_vp)]),
+    "vfkv_pages_destroy": (None, [_vp]),
+    "vfkv_pages_k_ptr": (_vp, [_vp]),
+    "vfkv_pages_v_ptr": (_vp, [_vp]),
+    "vfkv_pages_bytes_per_buffer": (_u64, [_vp]),
+    "vfkv_pages_offset_bytes": (_u64, [_vp, _u32, _u32]),
+    "vfkv_pages_free_count": (_u32, [_vp]),
+    "vfkv_pages_refcount": (_u32, [_vp, _u32]),
+    "vfkv_pages_alloc": (C.c_int, [_vp, _u32, _u32p]),
+    "vfkv_pages_retain": (C.c_int, [_vp, _u32p, _u32]),
+    "vfkv_pages_release": (C.c_int, [_vp, _u32p, _u32]),
+    "vfkv_pages_copy": (C.c_int, [_vp, _u32p, _u32p, _u32p, _u32, _vp]),
+    "vfkv_pages_fork": (C.c_int, [_vp, _u32p, _u32, _u32, _u32p, _vp]),
+    "vfkv_pages_compact": (C.c_int, [_vp, _u32p, _vp]),
+    "vfkv_paged_qk_rope_kv_write": (C.c_int, [_vp, _u32, C.POINTER(SeqBatchArgs), C.POINTER(PagedRows), C.POINTER(MRopeParams), _vp]),
+    "vfkv_paged_workspace_create": (C.c_int, [_vp, _u32, C.POINTER(_vp)]),
+    "vfkv_paged_decode_attention": (C.c_int, [_vp, _u32, C.POINTER(SeqBatchArgs), C.POINTER(PagedAttnParams), _vp, _vp, _vp, _vp]),
+    "vfkv_paged_prefill_attention": (C.c_int, [_vp, _u32, C.POINTER(SeqBatchArgs), C.POINTER(PagedAttnParams), _vp, _vp, _vp, _vp]),
     "vfkv_sigmoid_mul": (C.c_int, [C.POINTER(Gate), _vp, _u32, _vp]),
     "vfkv_decode_attention_gated": (C.c_int, [_vp, _u32, _u32, _u32, _vp, _vp, _vp, _vp, _u32, _u32, _f, _f, C.POINTER(Gate),
                                               _vp, _vp]),

@@ -12,6 +12,7 @@
 #include <vector>
 
 #include "../../include/vfkv.h"
+#include "api_internal.h"
 #include "device_utils.h"
 #include "kernels.h"
 
@@ -20,6 +21,13 @@ namespace {
 thread_local char g_err[512] = "";
 // Advisory of the last attention call on this thread (vfkv_last_note): never an error, never touches g_err.
 thread_local char g_note[256] = "";
+
+}  // namespace
+
+// Shared with the paged cache's entry points (paged_api.hip).
+namespace vfkv {
+
+void clear_note() { g_note[0] = '\0'; }
 
 void note_generic(const char* who, uint32_t dtype, uint32_t head_dim) {
     snprintf(g_note, sizeof(g_note), "%s: this shape (kv dtype %u, head_dim %u, or unaligned pointers / a layer slab of 2 GiB or more) "
@@ -37,6 +45,14 @@ int fail(int status, const char* fmt, ...) {
 int hip_fail(hipError_t e, const char* what) {
     return fail(e == hipErrorNoDevice ? VFKV_ERR_NO_DEVICE : VFKV_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
 }
+
+}  // namespace vfkv
+
+namespace {
+
+using vfkv::fail;
+using vfkv::hip_fail;
+using vfkv::note_generic;
 
 #define VFKV_HIP(call)                                  \
     do {                                                \
@@ -64,14 +80,6 @@ struct vfkv_cache {
     uint32_t current_seq_len;
 };
 
-struct vfkv_workspace {
-    uint32_t n_heads, head_dim, max_tiles;
-    float* scratch_out;
-    float* scratch_max;
-    float* scratch_sum;
-    float* q_rot;          // n_heads * head_dim floats: rotated queries of vfkv_qk_rope_kv_write_decode_attention when the caller
-                           // does not want them and the shape takes the separate RoPE launch
-};
 
 // Decode partials of vfkv_decode_attention_static: device memory that exists from the moment the library is loaded, so
 // the call needs no allocation.  Every GPU holds its own copy at its own address; host code never uses the array's

@@ -1,0 +1,22 @@
+// What the files of the C ABI share: error text, notes, the workspace object.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+struct vfkv_workspace {
+    uint32_t n_heads, head_dim, max_tiles;
+    float* scratch_out;
+    float* scratch_max;
+    float* scratch_sum;
+    float* q_rot;          // n_heads * head_dim floats: rotated queries of vfkv_qk_rope_kv_write_decode_attention when the caller
+                           // does not want them and the shape takes the separate RoPE launch
+};
+
+namespace vfkv {
+
+int fail(int status, const char* fmt, ...) __attribute__((format(printf, 2, 3)));   // sets the thread's error text, returns status
+int hip_fail(hipError_t e, const char* what);
+void clear_note();
+void note_generic(const char* who, uint32_t dtype, uint32_t head_dim);
+
+}  // namespace vfkv

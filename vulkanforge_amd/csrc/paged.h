@@ -1,0 +1,100 @@
+// Paged cache: what the kernels and the C ABI share (layout, batch of sequences, launch interface).
+//
+// K and V: [layer][page][kv_head][slot][d].  Position j of sequence s is slot j % page_size of page table[s][j / page_size]; the
+// page size is a power of two.  Lengths, offsets and page numbers come from device arrays that the host has not seen, so the
+// kernels bound every one of them before it becomes an address.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace vfkv {
+
+struct PagedSlab {             // one layer
+    const uint8_t* k;
+    const uint8_t* v;
+    uint64_t page_bytes;       // one page of one layer, one tensor
+    uint32_t n_pages, page_shift, n_kv_heads, head_dim, dtype;
+};
+struct PagedSeqs {
+    const int32_t* table;      // [n_seqs][table_stride]
+    const int32_t* kv_lens;    // [n_seqs]
+    const int32_t* q_offsets;  // [n_seqs + 1] or NULL: token t is the one token of sequence t
+    uint32_t n_seqs, table_stride, n_tokens;
+    uint32_t limit;            // min(table_stride * page_size, 2^31 - 1)
+};
+struct PagedAttnLaunch {
+    PagedSlab c;
+    PagedSeqs s;
+    const void* q = nullptr;
+    void* o = nullptr;
+    uint64_t q_stride = 0, o_stride = 0;   // elements between two tokens
+    uint32_t n_heads = 0, window = 0, n_sink = 0;
+    uint32_t io_f16 = 0;                   // q and o are f16 (else f32)
+    uint32_t max_kv = 0;                   // upper bound of the lengths that the host knows
+    float scale = 0.f, softcap = 0.f;
+    float* scratch_out = nullptr;          // partial outputs, maxima and sums of the parts of a sequence
+    float* scratch_max = nullptr;
+    float* scratch_sum = nullptr;
+    uint64_t scratch_rows = 0;             // partial rows (of head_dim floats) the scratch holds
+};
+struct PagedWriteLaunch {
+    PagedSlab c;
+    PagedSeqs s;
+    const void* q; const float* q_weight; void* q_out;
+    const void* k; const void* v; const float* k_weight;
+    const int32_t* positions; const float* freq_factors;
+    uint64_t q_stride, q_out_stride, k_stride, v_stride;
+    uint32_t n_heads, io_f16;
+    uint32_t mode, rotary_dim, n_axes, interleaved, section[4];
+    double log2_step;                      // log2 of the frequency ratio of neighbouring pairs: -2 log2(base) / rotary_dim
+    float freq_scale, attn_factor, eps;
+};
+constexpr uint32_t kCopyPairs = 256;       // page copies per launch: they travel as kernel arguments
+struct PagedCopyLaunch {
+    uint8_t* k;                            // whole buffers
+    uint8_t* v;
+    uint64_t layer_bytes, page_bytes;
+    uint32_t n_layers, n_kv_heads, page_size, row_bytes;   // row_bytes: one slot of one KV head
+    uint32_t n;
+    const uint32_t* src; const uint32_t* dst; const uint32_t* rows;   // host arrays, n <= kCopyPairs; rows NULL = all
+};
+
+hipError_t launch_paged_copy(const PagedCopyLaunch& L, hipStream_t stream);
+hipError_t launch_paged_write(const PagedWriteLaunch& L, hipStream_t stream);
+// One wavefront per (token, head): any head_dim <= 512, any alignment.
+hipError_t launch_paged_generic(const PagedAttnLaunch& L, hipStream_t stream);
+
+#ifdef __HIPCC__
+// Length of sequence s, within what its page table can hold.
+__device__ __forceinline__ uint32_t paged_kv_len(const PagedSeqs& S, uint32_t s) {
+    const int32_t n = S.kv_lens[s];
+    return n < 0 ? 0u : (uint32_t)n < S.limit ? (uint32_t)n : S.limit;
+}
+// Token rows [lo, hi) of sequence s.
+__device__ __forceinline__ void paged_rows(const PagedSeqs& S, uint32_t s, uint32_t& lo, uint32_t& hi) {
+    if (S.q_offsets == nullptr) { lo = s; hi = s + 1u; return; }
+    const int32_t a = S.q_offsets[s], b = S.q_offsets[s + 1u];
+    lo = a < 0 ? 0u : (uint32_t)a < S.n_tokens ? (uint32_t)a : S.n_tokens;
+    hi = b < 0 ? 0u : (uint32_t)b < S.n_tokens ? (uint32_t)b : S.n_tokens;
+    if (hi < lo) hi = lo;
+}
+// Sequence of token t (n_seqs when it has none): the first whose rows end behind t.
+__device__ __forceinline__ uint32_t paged_seq_of(const PagedSeqs& S, uint32_t t) {
+    if (S.q_offsets == nullptr) return t < S.n_seqs ? t : S.n_seqs;
+    uint32_t a = 0u, b = S.n_seqs;
+    while (a < b) {
+        const uint32_t mid = (a + b) >> 1;
+        if (S.q_offsets[mid + 1u] > (int32_t)t) b = mid; else a = mid + 1u;
+    }
+    return a < S.n_seqs && S.q_offsets[a] <= (int32_t)t ? a : S.n_seqs;
+}
+// Page of positions [i * page_size, (i + 1) * page_size) of sequence s; n_pages when there is none.
+__device__ __forceinline__ uint32_t paged_page(const PagedSlab& c, const PagedSeqs& S, uint32_t s, uint32_t i) {
+    const uint32_t p = (uint32_t)S.table[(uint64_t)s * S.table_stride + i];
+    return p < c.n_pages ? p : c.n_pages;
+}
+// First key of the window of the query at position p (keys in front of it are visible only as one of the first n_sink).
+__device__ __forceinline__ uint32_t paged_window_lo(uint32_t window, uint32_t p) { return window != 0u && p + 1u > window ? p + 1u - window : 0u; }
+#endif
+
+}  // namespace vfkv

@@ -23,7 +23,27 @@ use std::os::raw::{c_char, c_int, c_void};
 #[repr(C)] pub struct VfkvGate {                  // SigmoidMulPushConstants (runs.rs:2667) plus the gate buffer
     pub gate: *const f32, pub chunk: u32, pub stride: u32, pub gate_offset: u32,
 }
-pub enum VfkvCache {} pub enum VfkvWorkspace {}
+#[repr(C)] pub struct VfkvPagesConfig {           // paged cache (several sequences over one pool of pages)
+    pub n_layers: u32, pub n_kv_heads: u32, pub head_dim: u32, pub page_size: u32, pub n_pages: u32, pub dtype: u32,
+}
+#[repr(C)] pub struct VfkvSeqBatch {              // device arrays; q_offsets may be null (one token per sequence)
+    pub page_table: *const i32, pub kv_lens: *const i32, pub q_offsets: *const i32,
+    pub n_seqs: u32, pub table_stride: u32, pub n_tokens: u32, pub max_kv_len: u32,
+}
+#[repr(C)] pub struct VfkvMropeParams {
+    pub rope_mode: u32, pub rotary_dim: u32, pub n_axes: u32, pub interleaved: u32, pub section: [u32; 4],
+    pub freq_base: f32, pub freq_scale: f32, pub attn_factor: f32, pub eps: f32,
+}
+#[repr(C)] pub struct VfkvPagedRows {
+    pub q: *const c_void, pub q_norm_weight: *const f32, pub q_out: *mut c_void, pub k: *const c_void, pub v: *const c_void,
+    pub k_norm_weight: *const f32, pub positions: *const i32, pub freq_factors: *const f32,
+    pub n_heads: u32, pub io_dtype: u32, pub q_stride: u32, pub q_out_stride: u32, pub k_stride: u32, pub v_stride: u32,
+}
+#[repr(C)] pub struct VfkvPagedAttnParams {
+    pub n_heads: u32, pub window: u32, pub n_sink: u32, pub io_dtype: u32, pub q_stride: u32, pub o_stride: u32,
+    pub scale: f32, pub softcap: f32,
+}
+pub enum VfkvCache {} pub enum VfkvWorkspace {} pub enum VfkvPages {}
 extern "C" {
     pub fn vfkv_last_error() -> *const c_char;
     pub fn vfkv_last_note() -> *const c_char;
@@ -128,4 +148,31 @@ extern "C" {
                                         gate: *const VfkvGate, stream: *mut c_void) -> c_int;
     pub fn vfkv_flash_attn_batch(q: *const f32, k_layer: *const c_void, v_layer: *const c_void, kv_dtype: u32,
                                  o: *mut f32, p: *const VfkvBatchParams, softcap: f32, stream: *mut c_void) -> c_int;
+    pub fn vfkv_pages_create(cfg: *const VfkvPagesConfig, out: *mut *mut VfkvPages) -> c_int;
+    pub fn vfkv_pages_create_external(cfg: *const VfkvPagesConfig, k_buffer: *mut c_void, v_buffer: *mut c_void,
+                                      out: *mut *mut VfkvPages) -> c_int;
+    pub fn vfkv_pages_destroy(c: *mut VfkvPages);
+    pub fn vfkv_pages_k_ptr(c: *const VfkvPages) -> *mut c_void;
+    pub fn vfkv_pages_v_ptr(c: *const VfkvPages) -> *mut c_void;
+    pub fn vfkv_pages_bytes_per_buffer(c: *const VfkvPages) -> u64;
+    pub fn vfkv_pages_offset_bytes(c: *const VfkvPages, layer: u32, page: u32) -> u64;
+    pub fn vfkv_pages_free_count(c: *const VfkvPages) -> u32;
+    pub fn vfkv_pages_refcount(c: *const VfkvPages, page: u32) -> u32;
+    pub fn vfkv_pages_alloc(c: *mut VfkvPages, n: u32, pages_out: *mut u32) -> c_int;
+    pub fn vfkv_pages_retain(c: *mut VfkvPages, pages: *const u32, n: u32) -> c_int;
+    pub fn vfkv_pages_release(c: *mut VfkvPages, pages: *const u32, n: u32) -> c_int;
+    pub fn vfkv_pages_copy(c: *mut VfkvPages, src: *const u32, dst: *const u32, rows: *const u32, n: u32,
+                           stream: *mut c_void) -> c_int;               // host arrays
+    pub fn vfkv_pages_fork(c: *mut VfkvPages, pages: *const u32, kv_len: u32, n_forks: u32, pages_out: *mut u32,
+                           stream: *mut c_void) -> c_int;
+    pub fn vfkv_pages_compact(c: *mut VfkvPages, new_ids_out: *mut u32, stream: *mut c_void) -> c_int;
+    pub fn vfkv_paged_qk_rope_kv_write(c: *mut VfkvPages, layer: u32, b: *const VfkvSeqBatch, rows: *const VfkvPagedRows,
+                                       p: *const VfkvMropeParams, stream: *mut c_void) -> c_int;
+    pub fn vfkv_paged_workspace_create(c: *const VfkvPages, n_heads: u32, out: *mut *mut VfkvWorkspace) -> c_int;
+    pub fn vfkv_paged_decode_attention(c: *mut VfkvPages, layer: u32, b: *const VfkvSeqBatch, p: *const VfkvPagedAttnParams,
+                                       q: *const c_void, o: *mut c_void, ws: *mut VfkvWorkspace,
+                                       stream: *mut c_void) -> c_int;
+    pub fn vfkv_paged_prefill_attention(c: *mut VfkvPages, layer: u32, b: *const VfkvSeqBatch, p: *const VfkvPagedAttnParams,
+                                        q: *const c_void, o: *mut c_void, ws: *mut VfkvWorkspace,
+                                        stream: *mut c_void) -> c_int;
 }

@@ -1,0 +1,297 @@
+"""Host mirror of the paged cache: a pool of pages with reference counts, batches of sequences over it, and the calls that
+fill and read it (``include/vfkv.h``, section "Paged cache").
+
+Arguments are PyTorch device tensors; PyTorch only supplies memory and the stream.  Every compute method enqueues on
+``stream`` (default: torch's current stream on the cache's device) and returns without synchronising.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+from dataclasses import dataclass
+from typing import List, Optional, Sequence
+
+from . import _ffi
+from .forward import Workspace
+from .kv_cache import KvDtype
+
+NO_PAGE = -1     # an entry of a page list or page table without a page
+
+
+@dataclass
+class PagedKvConfig:
+    n_layers: int
+    n_kv_heads: int
+    head_dim: int
+    page_size: int
+    n_pages: int
+    dtype: KvDtype = KvDtype.F16
+
+
+def _pages(values: Sequence[int]):
+    """Page list -> uint32 array (-1 becomes VFKV_NO_PAGE)."""
+    return (C.c_uint32 * max(len(values), 1))(*[v & 0xFFFFFFFF for v in values])
+
+
+def _list(arr, n: int) -> List[int]:
+    return [NO_PAGE if v == _ffi.NO_PAGE else v for v in arr[:n]]
+
+
+def _stream(stream) -> int:
+    if stream is None:
+        import torch
+        return torch.cuda.current_stream().cuda_stream
+    return stream if isinstance(stream, int) else stream.cuda_stream
+
+
+class PagedKvCache:
+    """K and V as [layer][page][kv_head][slot][d], and the reference counts of the pages.
+
+    ``PagedKvCache(config)`` allocates on the current HIP device; ``k_buffer`` / ``v_buffer`` are device addresses of
+    caller-owned memory instead (keep it alive); ``layout_only=True`` builds the page counting without buffers."""
+
+    def __init__(self, config: PagedKvConfig, layout_only: bool = False, k_buffer: int = 0, v_buffer: int = 0):
+        L = _ffi.lib()
+        self.config = config
+        self.kv_dtype = KvDtype(config.dtype)
+        cfg = _ffi.PagesConfig(config.n_layers, config.n_kv_heads, config.head_dim, config.page_size, config.n_pages,
+                               int(config.dtype))
+        handle = C.c_void_p()
+        if layout_only or k_buffer or v_buffer:
+            _ffi.check(L.vfkv_pages_create_external(C.byref(cfg), k_buffer or None, v_buffer or None, C.byref(handle)))
+        else:
+            _ffi.check(L.vfkv_pages_create(C.byref(cfg), C.byref(handle)))
+        self._h = handle
+
+    def destroy(self) -> None:
+        if getattr(self, "_h", None):
+            _ffi.lib().vfkv_pages_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.destroy()
+        except Exception:
+            pass
+
+    @property
+    def handle(self):
+        return self._h
+
+    # -- layout --
+    @property
+    def k_ptr(self) -> int:
+        return int(_ffi.lib().vfkv_pages_k_ptr(self._h) or 0)
+
+    @property
+    def v_ptr(self) -> int:
+        return int(_ffi.lib().vfkv_pages_v_ptr(self._h) or 0)
+
+    def bytes_per_buffer(self) -> int:
+        return int(_ffi.lib().vfkv_pages_bytes_per_buffer(self._h))
+
+    def offset_bytes(self, layer: int, page: int) -> int:
+        return int(_ffi.lib().vfkv_pages_offset_bytes(self._h, layer, page))
+
+    def pages_for(self, kv_len: int) -> int:
+        """Pages a sequence of ``kv_len`` positions occupies."""
+        return -(-kv_len // self.config.page_size)
+
+    # -- page counting --
+    @property
+    def free_count(self) -> int:
+        return int(_ffi.lib().vfkv_pages_free_count(self._h))
+
+    def refcount(self, page: int) -> int:
+        return int(_ffi.lib().vfkv_pages_refcount(self._h, page & 0xFFFFFFFF))
+
+    def alloc(self, n: int) -> List[int]:
+        """The ``n`` lowest free pages; raises when fewer are free."""
+        out = (C.c_uint32 * max(n, 1))()
+        _ffi.check(_ffi.lib().vfkv_pages_alloc(self._h, n, out))
+        return list(out[:n])
+
+    def retain(self, pages: Sequence[int]) -> None:
+        _ffi.check(_ffi.lib().vfkv_pages_retain(self._h, _pages(pages), len(pages)))
+
+    def release(self, pages: Sequence[int]) -> None:
+        """One reference less per entry; pages without references are free (entries of -1 are skipped)."""
+        _ffi.check(_ffi.lib().vfkv_pages_release(self._h, _pages(pages), len(pages)))
+
+    # -- pages on the device --
+    def copy_pages(self, src: Sequence[int], dst: Sequence[int], rows: Optional[Sequence[int]] = None, stream=None) -> None:
+        """Copies page ``src[i]`` (its first ``rows[i]`` slots, default all) to page ``dst[i]``, all layers, K and V."""
+        if len(src) != len(dst) or (rows is not None and len(rows) != len(src)):
+            raise ValueError("src, dst and rows must have the same length")
+        _ffi.check(_ffi.lib().vfkv_pages_copy(self._h, _pages(src), _pages(dst), None if rows is None else _pages(rows),
+                                              len(src), _stream(stream)))
+
+    def fork(self, pages: Sequence[int], kv_len: int, n_forks: int, stream=None) -> List[List[int]]:
+        """Page lists of ``n_forks`` continuations of the sequence of ``kv_len`` positions in ``pages``: full pages are
+        shared, a last page that is not full is copied into a page of the fork's own."""
+        used = self.pages_for(kv_len)
+        if len(pages) < used:
+            raise ValueError(f"{kv_len} positions need {used} pages, got {len(pages)}")
+        out = (C.c_uint32 * max(used * n_forks, 1))()
+        _ffi.check(_ffi.lib().vfkv_pages_fork(self._h, _pages(pages[:used]), kv_len, n_forks, out,
+                                              _stream(stream) if self.k_ptr else None))
+        return [_list(out[i * used:(i + 1) * used], used) for i in range(n_forks)]
+
+    def compact(self, stream=None) -> List[int]:
+        """Moves the live pages into the lowest ids; returns every page's new id (-1: the page was free)."""
+        out = (C.c_uint32 * self.config.n_pages)()
+        _ffi.check(_ffi.lib().vfkv_pages_compact(self._h, out, _stream(stream) if self.k_ptr else None))
+        return _list(out, self.config.n_pages)
+
+
+def _int32(t, name: str):
+    import torch
+    if t.dtype is not torch.int32 or not t.is_cuda or not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous int32 device tensor")
+    return t
+
+
+class SeqBatch:
+    """Sequences of one call: ``page_table`` [n_seqs, entries], ``kv_lens`` [n_seqs] (this call's tokens included) and
+    ``q_offsets`` [n_seqs + 1] (None: one token per sequence), int32 device tensors.  The tensors are read when the
+    work runs, so one batch object serves every step that updates them in place, captured steps too; they are kept alive."""
+
+    def __init__(self, page_table, kv_lens, q_offsets=None, n_tokens: Optional[int] = None, max_kv_len: int = 0):
+        n = kv_lens.numel()
+        if page_table.dim() != 2 or page_table.shape[0] != n or kv_lens.dim() != 1:
+            raise ValueError("page_table must be [n_seqs, entries] and kv_lens [n_seqs]")
+        if q_offsets is not None and (q_offsets.dim() != 1 or q_offsets.numel() != n + 1):
+            raise ValueError("q_offsets must be [n_seqs + 1]")
+        if n_tokens is None:
+            if q_offsets is not None:
+                raise ValueError("n_tokens is needed with q_offsets (the offsets are on the device)")
+            n_tokens = n
+        devices = {t.device for t in (page_table, kv_lens, q_offsets) if t is not None}
+        if len(devices) != 1:
+            raise ValueError("page_table, kv_lens and q_offsets must be on one device")
+        self.page_table, self.kv_lens = _int32(page_table, "page_table"), _int32(kv_lens, "kv_lens")
+        self.q_offsets = None if q_offsets is None else _int32(q_offsets, "q_offsets")
+        self.n_seqs, self.n_tokens = n, n_tokens
+        self.device = kv_lens.device
+        self._args = _ffi.SeqBatchArgs(self.page_table.data_ptr(), self.kv_lens.data_ptr(),
+                                       None if q_offsets is None else self.q_offsets.data_ptr(), n, page_table.shape[1],
+                                       n_tokens, max_kv_len)
+        self.args = C.byref(self._args)
+
+
+class MRope:
+    """Rotation of rows whose tokens have positions on one to four axes (time, height, width, ...): ``sections[a]`` pairs
+    of axis ``a``, in blocks or ``interleaved``.  ``rotary_dim=0``: none."""
+
+    def __init__(self, rotary_dim: int, freq_base: float = 10000.0, sections: Optional[Sequence[int]] = None,
+                 interleaved: bool = False, rope_mode: int = _ffi.ROPE_NEOX, freq_scale: float = 1.0,
+                 attn_factor: float = 1.0, eps: float = 1e-6):
+        sections = [rotary_dim // 2] if sections is None else list(sections)
+        if not 1 <= len(sections) <= 4:
+            raise ValueError("1 to 4 axes")
+        self.n_axes = len(sections)
+        self._args = _ffi.MRopeParams(rope_mode, rotary_dim, self.n_axes, int(interleaved),
+                                      (C.c_uint32 * 4)(*(sections + [0] * (4 - self.n_axes))), freq_base, freq_scale,
+                                      attn_factor, eps)
+        self.args = C.byref(self._args)
+
+
+class PagedWorkspace(Workspace):
+    """Scratch of the paged attention calls for one cache geometry, whatever the batch."""
+
+    def __init__(self, cache: PagedKvCache, n_heads: int):
+        h = C.c_void_p()
+        _ffi.check(_ffi.lib().vfkv_paged_workspace_create(cache.handle, n_heads, C.byref(h)))
+        self._h = h
+
+    @property
+    def handle(self):
+        return self._h
+
+
+class PagedForward:
+    """The calls of one model over a paged cache: its query heads, a workspace, and ``attn_scale = 1/sqrt(head_dim)``.
+
+    Rows are [n_tokens, heads, head_dim] tensors, f32 or f16, contiguous within a token; tokens may be apart (a slice of
+    one projection's output)."""
+
+    def __init__(self, cache: PagedKvCache, n_heads: int, workspace: Optional[PagedWorkspace] = None):
+        self.cache, self.n_heads = cache, n_heads
+        self.workspace = workspace or PagedWorkspace(cache, n_heads)
+        self.attn_scale = 1.0 / math.sqrt(cache.config.head_dim)
+
+    def _rows(self, t, heads: int, batch: SeqBatch, name: str):
+        """(address, elements between two tokens, io dtype) of a row tensor."""
+        if t.dim() != 3 or t.shape[0] != batch.n_tokens or t.shape[1] != heads or t.shape[2] != self.cache.config.head_dim:
+            raise ValueError(f"{name}: expected [{batch.n_tokens}, {heads}, {self.cache.config.head_dim}], got {list(t.shape)}")
+        if t.device != batch.device:
+            raise ValueError(f"{name} is on {t.device}, the batch on {batch.device}")
+        d = t.element_size()
+        if d == 4:
+            io = 0
+        elif d == 2:
+            io = 1
+        else:
+            io = -1
+        if io < 0 or str(t.dtype) != ("torch.float32", "torch.float16")[io]:
+            raise ValueError(f"{name}: float32 or float16, got {t.dtype}")
+        token, head, elem = t.stride()
+        if (elem != 1 and t.shape[2] > 1) or (head != t.shape[2] and heads > 1):
+            raise ValueError(f"{name}: the heads of a token must be contiguous")
+        if t.shape[0] <= 1:
+            token = heads * t.shape[2]
+        if not heads * t.shape[2] <= token <= 0xFFFFFFFF:
+            raise ValueError(f"{name}: tokens overlap or are too far apart (stride {token})")
+        return t.data_ptr(), token, io
+
+    def _dev(self, t, shape, dtype: str, batch: SeqBatch, name: str) -> Optional[int]:
+        if t is None:
+            return None
+        if tuple(t.shape) != shape or str(t.dtype) != dtype or not t.is_contiguous() or t.device != batch.device:
+            raise ValueError(f"{name}: expected a contiguous {dtype} tensor of shape {shape} on {batch.device}")
+        return t.data_ptr()
+
+    def qk_rope_kv_write(self, layer: int, batch: SeqBatch, q, k, v, rope: MRope, q_out=None, q_norm_weight=None,
+                         k_norm_weight=None, positions=None, freq_factors=None, stream=None) -> None:
+        """Norm (with a weight) and rotation of the query rows into ``q_out`` (default: in place) and of the key rows,
+        and the append of keys and values at their tokens' positions.  ``q`` may be None.  ``positions``
+        [n_axes, n_tokens] int32 (default: every axis has the token's position in its sequence)."""
+        cfg = self.cache.config
+        kp, ks, io = self._rows(k, cfg.n_kv_heads, batch, "k")
+        vp, vs, iov = self._rows(v, cfg.n_kv_heads, batch, "v")
+        qp = qs = op = os_ = None
+        ioq = ioo = io
+        if q is not None:
+            qp, qs, ioq = self._rows(q, self.n_heads, batch, "q")
+            op, os_, ioo = (qp, qs, ioq) if q_out is None else self._rows(q_out, self.n_heads, batch, "q_out")
+        if not io == iov == ioq == ioo:
+            raise ValueError("q, k, v and q_out must have one dtype")
+        half = rope._args.rotary_dim // 2
+        r = _ffi.PagedRows(qp, self._dev(q_norm_weight, (cfg.head_dim,), "torch.float32", batch, "q_norm_weight"), op, kp, vp,
+                           self._dev(k_norm_weight, (cfg.head_dim,), "torch.float32", batch, "k_norm_weight"),
+                           self._dev(positions, (rope.n_axes, batch.n_tokens), "torch.int32", batch, "positions"),
+                           self._dev(freq_factors, (half,), "torch.float32", batch, "freq_factors"),
+                           self.n_heads, io, qs or 0, os_ or 0, ks, vs)
+        _ffi.check(_ffi.lib().vfkv_paged_qk_rope_kv_write(self.cache.handle, layer, batch.args, C.byref(r), rope.args,
+                                                          _stream(stream)))
+
+    def _attention(self, fn, layer, batch, q, o, window, n_sink, scale, softcap, stream) -> None:
+        qp, qs, io = self._rows(q, self.n_heads, batch, "q")
+        op, os_, ioo = self._rows(o, self.n_heads, batch, "o")
+        if io != ioo:
+            raise ValueError("q and o must have one dtype")
+        if window < 0 or n_sink < 0:
+            raise ValueError("window and n_sink must not be negative")
+        p = _ffi.PagedAttnParams(self.n_heads, window, n_sink, io, qs, os_, self.attn_scale if scale is None else scale, softcap)
+        _ffi.check(fn(self.cache.handle, layer, batch.args, C.byref(p), qp, op, self.workspace.handle, _stream(stream)))
+
+    def decode_attention(self, layer: int, batch: SeqBatch, q, o, window: int = 0, n_sink: int = 0,
+                         scale: Optional[float] = None, softcap: float = 0.0, stream=None) -> None:
+        """One token per sequence (a batch without ``q_offsets``) over the keys it sees: all, or the last ``window`` ones
+        and the first ``n_sink``."""
+        self._attention(_ffi.lib().vfkv_paged_decode_attention, layer, batch, q, o, window, n_sink, scale, softcap, stream)
+
+    def prefill_attention(self, layer: int, batch: SeqBatch, q, o, window: int = 0, n_sink: int = 0,
+                          scale: Optional[float] = None, softcap: float = 0.0, stream=None) -> None:
+        """Causal attention of every sequence's tokens; the window is each query's own."""
+        self._attention(_ffi.lib().vfkv_paged_prefill_attention, layer, batch, q, o, window, n_sink, scale, softcap, stream)
