@@ -539,7 +539,7 @@ typedef struct vfkv_seq_batch {
     const int32_t* page_table; /* [n_seqs][table_stride] */
     const int32_t* kv_lens;    /* [n_seqs] */
     const int32_t* q_offsets;  /* [n_seqs + 1], not decreasing, or NULL: one token per sequence */
-    uint32_t n_seqs;           /* <= 8192 */
+    uint32_t n_seqs;           /* <= 4096 */
     uint32_t table_stride;     /* page table entries per sequence */
     uint32_t n_tokens;         /* rows of q / k / v / o */
     uint32_t max_kv_len;       /* upper bound of kv_lens that sizes the launch (0: none known).  Results do not depend on it. */

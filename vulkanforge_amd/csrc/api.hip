@@ -561,7 +561,8 @@ int vfkv_workspace_create(uint32_t n_heads, uint32_t head_dim, uint32_t max_seq_
     const uint64_t out_b = (n_out * 4u + 255u) & ~255ull, ml_b = (n_ml * 4u + 255u) & ~255ull;
     void* base = nullptr;
     const uint64_t q_b = ((uint64_t)n_heads * head_dim * 4u + 255u) & ~255ull;
-    hipError_t e = hipMalloc(&base, out_b + 2u * ml_b + q_b);
+    hipError_t e = hipGetDevice(&w->device);
+    if (e == hipSuccess) e = hipMalloc(&base, out_b + 2u * ml_b + q_b);
     if (e != hipSuccess) { delete w; return hip_fail(e, "hipMalloc(workspace)"); }
     w->scratch_out = (float*)base;
     w->scratch_max = (float*)((char*)base + out_b);

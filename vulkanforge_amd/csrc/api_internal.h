@@ -5,6 +5,7 @@
 
 struct vfkv_workspace {
     uint32_t n_heads, head_dim, max_tiles;
+    int device;            // where the scratch is
     float* scratch_out;
     float* scratch_max;
     float* scratch_sum;

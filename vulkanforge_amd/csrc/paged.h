@@ -49,6 +49,7 @@ struct PagedWriteLaunch {
     double log2_step;                      // log2 of the frequency ratio of neighbouring pairs: -2 log2(base) / rotary_dim
     float freq_scale, attn_factor, eps;
 };
+constexpr uint32_t kPagedMaxSeqs = 4096;   // sequences per call: their unit counts are summed in LDS
 constexpr uint32_t kCopyPairs = 256;       // page copies per launch: they travel as kernel arguments
 struct PagedCopyLaunch {
     uint8_t* k;                            // whole buffers
@@ -61,6 +62,12 @@ struct PagedCopyLaunch {
 
 hipError_t launch_paged_copy(const PagedCopyLaunch& L, hipStream_t stream);
 hipError_t launch_paged_write(const PagedWriteLaunch& L, hipStream_t stream);
+// Matrix-core kernels: head_dim a multiple of 16 up to 256; q and o 16-byte aligned with strides that keep every row so
+// (paged_rows_aligned).
+hipError_t launch_paged_decode(const PagedAttnLaunch& L, hipStream_t stream);
+// Workgroups per head group (KV head and slice of its query heads) the decode launch may use: its scratch holds two partial
+// rows per workgroup and head.
+uint32_t paged_decode_wgs(uint32_t head_groups);
 // One wavefront per (token, head): any head_dim <= 512, any alignment.
 hipError_t launch_paged_generic(const PagedAttnLaunch& L, hipStream_t stream);
 

@@ -70,7 +70,7 @@ int check_batch(const vfkv_pages* c, const vfkv_seq_batch* b, const char* who, v
     if (!b->page_table || !b->kv_lens) return fail(VFKV_ERR_INVALID_ARG, "%s: NULL page table or lengths", who);
     if ((((uintptr_t)b->page_table | (uintptr_t)b->kv_lens | (uintptr_t)b->q_offsets) & 3u) != 0u)
         return fail(VFKV_ERR_ALIGNMENT, "%s: the batch's arrays must be 4-byte aligned", who);
-    if (b->n_seqs > 8192u) return fail(VFKV_ERR_UNSUPPORTED, "%s: %u sequences (at most 8192 in one call)", who, b->n_seqs);
+    if (b->n_seqs > vfkv::kPagedMaxSeqs) return fail(VFKV_ERR_UNSUPPORTED, "%s: %u sequences (at most %u in one call)", who, b->n_seqs, vfkv::kPagedMaxSeqs);
     if (b->table_stride == 0u) return fail(VFKV_ERR_INVALID_ARG, "%s: table_stride must be > 0", who);
     if (b->n_tokens > 0x7FFFFFFFu) return fail(VFKV_ERR_UNSUPPORTED, "%s: %u tokens", who, b->n_tokens);
     if (!b->q_offsets && b->n_tokens != b->n_seqs)
@@ -100,6 +100,8 @@ int row_stride(uint32_t given, uint64_t row, const char* who, const char* what, 
     *out = given ? given : row;
     return VFKV_OK;
 }
+
+constexpr uint64_t kPrefillRows = 65536;       // partial rows a paged workspace has at least
 
 int check_io(uint32_t io, const char* who) {
     if (io != VFKV_F32 && io != VFKV_F16) return fail(VFKV_ERR_INVALID_ARG, "%s: io_dtype %u (F32 and F16 are built)", who, io);
@@ -427,7 +429,10 @@ int vfkv_paged_workspace_create(const vfkv_pages* c, uint32_t n_heads, vfkv_work
     if (!c) return fail(VFKV_ERR_INVALID_ARG, "paged_workspace: cache is NULL");
     if (n_heads == 0u || n_heads % c->cfg.n_kv_heads != 0u)
         return fail(VFKV_ERR_INVALID_ARG, "n_heads (%u) is not a multiple of n_kv_heads (%u)", n_heads, c->cfg.n_kv_heads);
-    const uint64_t tiles = 64u;
+    // rows of head_dim floats: two per head and workgroup of the decode launch, and room for the prefill's split over the keys
+    const uint32_t slices = (n_heads / c->cfg.n_kv_heads + 7u) / 8u;
+    uint64_t tiles = 2u * (uint64_t)vfkv::paged_decode_wgs(c->cfg.n_kv_heads * slices);
+    if (tiles < kPrefillRows / n_heads) tiles = kPrefillRows / n_heads;
     return vfkv_workspace_create(n_heads, c->cfg.head_dim, (uint32_t)(tiles * 64u), out);
 }
 
@@ -463,9 +468,21 @@ static int paged_attention(vfkv_pages* c, uint32_t layer, const vfkv_seq_batch* 
     L.q = q; L.o = o;
     L.n_heads = p->n_heads; L.window = p->window; L.n_sink = p->n_sink; L.io_f16 = p->io_dtype == VFKV_F16;
     L.scale = p->scale; L.softcap = p->softcap;
+    if (ws) {
+        if ((rc = check_device(ws->device, who, "workspace")) != VFKV_OK) return rc;
+        L.scratch_out = ws->scratch_out; L.scratch_max = ws->scratch_max; L.scratch_sum = ws->scratch_sum;
+        // (rows of this call's head_dim: the workspace may have been made for wider ones)
+        L.scratch_rows = (uint64_t)ws->n_heads * ws->max_tiles;
+    }
     vfkv::clear_note();
-    VFKV_HIP(vfkv::launch_paged_generic(L, S(stream)));
-    vfkv::note_generic(who, c->cfg.dtype, hd);
+    const uint32_t per16 = p->io_dtype == VFKV_F32 ? 4u : 8u;
+    const bool aligned = (((uintptr_t)q | (uintptr_t)o) & 15u) == 0u && L.q_stride % per16 == 0u && L.o_stride % per16 == 0u;
+    if (hd % 16u != 0u || hd > 256u || !aligned || !decode) {
+        VFKV_HIP(vfkv::launch_paged_generic(L, S(stream)));
+        vfkv::note_generic(who, c->cfg.dtype, hd);
+        return VFKV_OK;
+    }
+    VFKV_HIP(vfkv::launch_paged_decode(L, S(stream)));
     return VFKV_OK;
 }
 

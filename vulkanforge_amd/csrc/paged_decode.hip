@@ -1,0 +1,614 @@
+// Decode attention over the paged cache: one token per sequence, a batch of sequences of any lengths.
+//
+// o = sum_j softmax_j(scale q.k_j) v_j per head; bound by reading K and V once (4 flop per element and query head against 1, 2 or 4
+// bytes), so the kernel is built around keeping loads in flight on every CU whatever the lengths are:
+//
+//   - The keys of ALL sequences, cut into units of 16 * SUB aligned positions (first tokens, then the window), are one line of U
+//     units per KV head.  Workgroup w of N owns units [w U / N, (w + 1) U / N): every workgroup has the same work to one unit, a
+//     long sequence is spread over many workgroups and short ones are packed.  A workgroup's range touches at most two
+//     sequences partly (its first and its last); those parts leave unnormalised sums that paged_merge_kernel joins, sequences
+//     inside the range are written directly.  The lengths are device data, so each workgroup finds its range itself
+//     (a prefix sum over the batch in LDS).
+//   - The four wavefronts of a workgroup take the units of a sequence in turn.  A 16-key tile lies in one page (page sizes are
+//     multiples of 16), so a page number is one scalar load, requested two units ahead; K and V rows go from memory to
+//     registers one unit ahead.
+//   - Both products run on the matrix cores, transposed, so that no register changes lanes in between:
+//       S^T[key, col] = K Q^T: A = K rows as loaded (FP8 widened exactly), B = Q^T.  Columns 0-7 hold f16(q'), columns 8-15
+//         f16(q' - f16(q')) of the same heads (q' = q * scale * log2 e): the sum of both columns has f32-level accuracy.
+//       O^T[d, col] += V^T P^T: B = P as the score tile left it (a lane holds four consecutive keys of one column, which is what
+//         the operand wants when the contraction runs over the keys in that order), columns 0-7 f16(p), 8-15 the remainder.
+//         A = V^T: a lane loads D / 16 columns of its four keys per tile and turns that small matrix with byte permutes
+//         in its own registers -- no LDS, no barrier.
+//     F32 caches use the f32 matrix instruction with the same ownership; nothing needs turning there.
+//   - The running maximum is only raised when a score exceeds it by 2^8: weights are kept times 2^6 (at most 2^14 in f16, smallest
+//     step 2^-30 of the largest), and the accumulators are rescaled a few times per sequence instead of once per unit.
+#include "device_utils.h"
+#include "paged.h"
+
+namespace vfkv {
+
+namespace {
+
+constexpr int kDecWaves = 4;
+constexpr int kDecHeads = 8;               // query heads of a KV head per workgroup
+constexpr float kRaise = 8.f, kBias = 6.f;  // log2
+
+template <int DT, int D, int SUB_>
+struct DecShape {
+    static constexpr int ES = DT == kF32 ? 4 : DT == kF16 ? 2 : 1;
+    static constexpr int SUB = SUB_;                     // 16-key tiles per unit
+    static constexpr int UK = 16 * SUB;                  // keys per unit
+    static constexpr int KE = 16 / ES;                   // elements of a 16-byte piece of a K row
+    static constexpr int KL = D / (4 * KE);              // pieces per lane and row: piece x of lane group g is elements (4 x + g) KE ..
+    static constexpr int NT = D / 16;                    // d-tiles = V elements per lane and key
+    static constexpr int PE = NT < KE ? NT : KE;         // elements of a V piece: piece y of lane r is elements (16 y + r) PE ..
+    static constexpr int VP = NT / PE;                   // V pieces
+    static constexpr int PW = PE * ES / 4;               // dwords of a V piece
+    static constexpr int VW = VP * PW;                   // V dwords per lane and key
+};
+
+// Units of a sequence of n keys: first tokens, then the window of the query at position n - 1.
+struct SeqUnits {
+    uint32_t n, lo, sink, sink_units, first, units;
+};
+__device__ __forceinline__ SeqUnits seq_units(uint32_t n, uint32_t window, uint32_t n_sink, uint32_t uk) {
+    SeqUnits r;
+    r.n = n;
+    r.lo = n ? paged_window_lo(window, n - 1u) : 0u;
+    r.sink = n_sink < r.lo ? n_sink : r.lo;
+    r.first = r.lo / uk;
+    const uint32_t su = (r.sink + uk - 1u) / uk;
+    r.sink_units = su < r.first ? su : r.first;         // what reaches the window's first unit belongs to it
+    r.units = n ? r.sink_units + (n + uk - 1u) / uk - r.first : 0u;
+    return r;
+}
+
+// Workgroups that share U units: the launch's, or as many as get two units per wavefront.  Never more than U, so that no range is
+// empty; 0 for an empty batch.
+__device__ __forceinline__ uint32_t used_wgs(uint32_t U, uint32_t n_wg) {
+    const uint32_t most = (U + 2u * kDecWaves - 1u) / (2u * kDecWaves);
+    return most < n_wg ? most : n_wg;
+}
+
+__device__ __forceinline__ float max_over_groups(float x) {   // over lanes with the same lane & 15
+    float y = x;
+    swap16(x, y);
+    x = fmaxf(x, y);
+    y = x;
+    swap32(x, y);
+    return fmaxf(x, y);
+}
+__device__ __forceinline__ float sum_over_groups(float x) { return xor32_sum(xor16_sum(x)); }
+__device__ __forceinline__ float ror8_sum(float x) { return x + dpp_f<kDppRor8>(x); }   // columns c and c + 8
+
+}  // namespace
+
+// Prefix sums of the units: pre[s] for s <= n_seqs, by the whole workgroup.
+template <int UK>
+__device__ __forceinline__ void unit_prefix(const PagedAttnLaunch& a, uint32_t* pre, uint32_t* wave_sum, int tid) {
+    const int lane = tid & 63, w = tid >> 6;
+    uint32_t carry = 0u;
+    for (uint32_t base = 0; base < a.s.n_seqs; base += 256u) {
+        const uint32_t s = base + (uint32_t)tid;
+        uint32_t x = s < a.s.n_seqs ? seq_units(paged_kv_len(a.s, s), a.window, a.n_sink, UK).units : 0u;
+        const uint32_t mine = x;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const uint32_t y = __shfl_up(x, off, kWave);
+            if (lane >= off) x += y;
+        }
+        if (lane == 63) wave_sum[w] = x;
+        __syncthreads();
+        uint32_t before = carry;
+#pragma unroll
+        for (int i = 0; i < kDecWaves; ++i) {
+            if (i < w) before += wave_sum[i];
+            carry += wave_sum[i];
+        }
+        if (s < a.s.n_seqs) pre[s] = before + x - mine;
+        __syncthreads();
+    }
+    if (tid == 0) pre[a.s.n_seqs] = carry;
+    __syncthreads();
+}
+
+template <int DT, int D, int SUB>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_decode_kernel(PagedAttnLaunch a, uint32_t n_wg, uint32_t slices) {
+    using Z = DecShape<DT, D, SUB>;
+    constexpr int OP = D + 4;                                            // pitch of an output row in LDS
+    __shared__ __attribute__((aligned(16))) float o_lds[kDecWaves][kDecHeads][OP];
+    __shared__ float m_lds[kDecWaves][kDecHeads], l_lds[kDecWaves][kDecHeads];
+    __shared__ uint32_t wave_sum[kDecWaves];
+    extern __shared__ uint32_t pre[];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n16 = lane & 15, g = lane >> 4, col = n16 & 7;
+    const bool is_lo = n16 >= 8;
+    const uint32_t wg = blockIdx.y;
+    const uint32_t kvh = blockIdx.x / slices, slice = blockIdx.x - kvh * slices;
+    const uint32_t group = a.n_heads / a.c.n_kv_heads;
+    const uint32_t h0 = kvh * group + slice * kDecHeads;
+    const uint32_t heads = group - slice * kDecHeads < (uint32_t)kDecHeads ? group - slice * kDecHeads : (uint32_t)kDecHeads;
+    const uint32_t dr = a.c.head_dim;
+    unit_prefix<Z::UK>(a, pre, wave_sum, tid);
+    const uint32_t U = pre[a.s.n_seqs];
+    // sequences without a key: zeros
+    for (uint32_t s = wg; s < a.s.n_seqs; s += n_wg) {
+        if (pre[s + 1u] != pre[s]) continue;
+        for (uint32_t e = tid; e < heads * dr; e += 256u) {
+            const uint64_t at = (uint64_t)s * a.o_stride + (uint64_t)h0 * dr + e;
+            if (a.io_f16) reinterpret_cast<_Float16*>(a.o)[at] = (_Float16)0.f; else reinterpret_cast<float*>(a.o)[at] = 0.f;
+        }
+    }
+    const uint32_t n_eff = used_wgs(U, n_wg);
+    if (wg >= n_eff) return;
+    const uint32_t u0 = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)wg * U / n_eff));
+    const uint32_t u1 = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)(wg + 1u) * U / n_eff));
+    uint32_t s_first;
+    {
+        uint32_t x = 0u, y = a.s.n_seqs - 1u;                            // the last s with pre[s] <= u0 (it has units)
+        while (x < y) {
+            const uint32_t mid = (x + y + 1u) >> 1;
+            if (pre[mid] <= u0) x = mid; else y = mid - 1u;
+        }
+        s_first = __builtin_amdgcn_readfirstlane(x);
+    }
+    const float scale_l2 = a.scale * 1.44269504088896f;
+    const float cap_l2 = a.softcap * 1.44269504088896f;
+    const float inv_cap_l2 = a.softcap > 0.f ? 1.0f / cap_l2 : 0.f;
+    // lane parts of the row addresses (pieces past a narrower head read its first piece again: they meet zeros of q, or are not stored)
+    const uint32_t row_b = dr * Z::ES;
+    uint32_t koff[Z::KL], voff[Z::VP];
+#pragma unroll
+    for (int x = 0; x < Z::KL; ++x) {
+        const uint32_t e = (uint32_t)(4 * x + g) * Z::KE;
+        koff[x] = (uint32_t)n16 * row_b + (e < dr ? e * Z::ES : 0u);
+    }
+#pragma unroll
+    for (int y = 0; y < Z::VP; ++y) {
+        const uint32_t e = (uint32_t)(16 * y + n16) * Z::PE;
+        voff[y] = 4u * (uint32_t)g * row_b + (e < dr ? e * Z::ES : 0u);
+    }
+    const uint64_t head_b = (uint64_t)kvh << a.c.page_shift;             // rows in front of this head's in a page
+    const uint32_t slot_mask = (1u << a.c.page_shift) - 1u;
+
+    struct Stage {
+        u32x4 k[SUB][Z::KL];
+        uint32_t v[SUB][4][Z::VW];
+    };
+    struct Pages {
+        uint32_t p[SUB];
+    };
+
+    for (uint32_t s = s_first; s < a.s.n_seqs; ++s) {
+        const uint32_t ps = __builtin_amdgcn_readfirstlane(pre[s]), pe = __builtin_amdgcn_readfirstlane(pre[s + 1u]);
+        if (ps >= u1) break;
+        if (ps == pe) continue;
+        const SeqUnits Q = seq_units(__builtin_amdgcn_readfirstlane(paged_kv_len(a.s, s)), a.window, a.n_sink, Z::UK);
+        const uint32_t ua = (ps > u0 ? ps : u0) - ps, ub = (pe < u1 ? pe : u1) - ps;   // units [ua, ub) of the sequence
+        const int32_t* const table = a.s.table + (uint64_t)s * a.s.table_stride;
+
+        // ---- q' as the B operand of the first product
+        half8_t qb[DT == kF32 ? 1 : D / 32];
+        float qf[DT == kF32 ? D / 4 : 1];
+        {
+            const bool there = (uint32_t)col < heads && (DT != kF32 || !is_lo);
+            const uint64_t qrow = (uint64_t)s * a.q_stride + (uint64_t)(h0 + (there ? (uint32_t)col : 0u)) * dr;
+            auto load8 = [&](uint32_t d, float* out, int n) {             // n = 4 or 8 elements of the head's row, times scale
+                const bool ok = there && d < dr;
+                const uint64_t at = qrow + (ok ? d : 0u);
+                for (int j = 0; j < n; j += 4) {
+                    float x[4];
+                    if (a.io_f16) {
+                        const half4_t h = *reinterpret_cast<const half4_t*>(reinterpret_cast<const _Float16*>(a.q) + at + j);
+                        for (int i = 0; i < 4; ++i) x[i] = (float)h[i];
+                    } else {
+                        const float4_t f = *reinterpret_cast<const float4_t*>(reinterpret_cast<const float*>(a.q) + at + j);
+                        for (int i = 0; i < 4; ++i) x[i] = f[i];
+                    }
+                    for (int i = 0; i < 4; ++i) out[j + i] = ok ? x[i] * scale_l2 : 0.f;
+                }
+            };
+            if constexpr (DT == kF32) {
+#pragma unroll
+                for (int x = 0; x < Z::KL; ++x) load8((uint32_t)(4 * x + g) * 4u, &qf[4 * x], 4);
+            } else {
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) {
+                    constexpr int PER = Z::KE / 8;                       // operands per piece
+                    float x[8];
+                    load8((uint32_t)(4 * (c / PER) + g) * Z::KE + 8u * (uint32_t)(c % PER), x, 8);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const _Float16 hi = (_Float16)x[j];
+                        qb[c][j] = is_lo ? (_Float16)(x[j] - (float)hi) : hi;
+                    }
+                }
+            }
+        }
+
+        float4_t acc[Z::NT];
+#pragma unroll
+        for (int n = 0; n < Z::NT; ++n) acc[n] = float4_t{0.f, 0.f, 0.f, 0.f};
+        float m = kMasked, l = 0.f;                                      // l: this lane's keys only, summed at the end
+
+        auto unit_key = [&](uint32_t u) { return (u < Q.sink_units ? u : Q.first + u - Q.sink_units) * (uint32_t)Z::UK; };
+        auto get_pages = [&](uint32_t u) {
+            Pages r;
+            const uint32_t kb = unit_key(u < ub ? u : ub - 1u);
+#pragma unroll
+            for (int t = 0; t < SUB; ++t) {
+                const uint32_t key = kb + 16u * t;
+                r.p[t] = (uint32_t)table[(key < Q.n ? key : Q.n - 1u) >> a.c.page_shift];
+            }
+            return r;
+        };
+        auto load = [&](Stage& st, const Pages& P, uint32_t u) {         // past the end: the last unit again, from the cache
+            const uint32_t kb = unit_key(u < ub ? u : ub - 1u);
+#pragma unroll
+            for (int t = 0; t < SUB; ++t) {
+                const uint32_t key = kb + 16u * t;
+                const uint32_t page = P.p[t] < a.c.n_pages ? P.p[t] : 0u;
+                // (a tile past the last key reads the page of the last key, inside the page: masked below)
+                const uint64_t off = (uint64_t)page * a.c.page_bytes + (head_b + (key & slot_mask)) * row_b;
+                const uint8_t* const kp = a.c.k + off;
+                const uint8_t* const vp = a.c.v + off;
+#pragma unroll
+                for (int x = 0; x < Z::KL; ++x) st.k[t][x] = *reinterpret_cast<const u32x4*>(kp + koff[x]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int y = 0; y < Z::VP; ++y) {
+                        const uint8_t* const src = vp + (voff[y] + (uint32_t)i * row_b);
+                        if constexpr (Z::PW == 4) {
+                            const u32x4 x = *reinterpret_cast<const u32x4*>(src);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) st.v[t][i][4 * y + e] = x[e];
+                        } else if constexpr (Z::PW == 2) {
+                            const u32x2 x = *reinterpret_cast<const u32x2*>(src);
+                            st.v[t][i][2 * y] = x[0];
+                            st.v[t][i][2 * y + 1] = x[1];
+                        } else {
+                            st.v[t][i][y] = *reinterpret_cast<const uint32_t*>(src);
+                        }
+                    }
+            }
+        };
+        auto compute = [&](Stage& st, const Pages& P, uint32_t u) {
+            const uint32_t kb = unit_key(u);
+            bool full = kb + (uint32_t)Z::UK <= Q.n && (kb >= Q.lo || kb + (uint32_t)Z::UK <= Q.sink);
+#pragma unroll
+            for (int t = 0; t < SUB; ++t) full = full && P.p[t] < a.c.n_pages;
+            float x[SUB][4];
+#pragma unroll
+            for (int t = 0; t < SUB; ++t) {
+                float4_t sc = {0.f, 0.f, 0.f, 0.f};
+                if constexpr (DT == kF32) {
+#pragma unroll
+                    for (int p = 0; p < Z::KL; ++p) {
+                        const float4_t kf = __builtin_bit_cast(float4_t, st.k[t][p]);   // (whole: a bit_cast of one element reads element 0)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) sc = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j], qf[4 * p + j], sc, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[t][i] = sc[i];
+                } else {
+#pragma unroll
+                    for (int c = 0; c < D / 32; ++c) {
+                        half8_t ka;
+                        if constexpr (DT == kF16) {
+                            ka = __builtin_bit_cast(half8_t, st.k[t][c]);
+                        } else {
+                            half2_t h[4];
+                            e4m3x4_to_h2(st.k[t][c / 2][2 * (c % 2)], h[0], h[1]);
+                            e4m3x4_to_h2(st.k[t][c / 2][2 * (c % 2) + 1], h[2], h[3]);
+                            ka = __builtin_bit_cast(half8_t, h);
+                        }
+                        sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qb[c], sc, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[t][i] = ror8_sum(sc[i]);
+                }
+            }
+            if (a.softcap > 0.f) {
+#pragma unroll
+                for (int t = 0; t < SUB; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[t][i] = softcap_l2(x[t][i], cap_l2, inv_cap_l2);
+            }
+            if (!full) {
+#pragma unroll
+                for (int t = 0; t < SUB; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t key = kb + 16u * t + 4u * (uint32_t)g + (uint32_t)i;
+                        const bool seen = key < Q.n && (key >= Q.lo || key < Q.sink) && P.p[t] < a.c.n_pages;
+                        x[t][i] = seen ? x[t][i] : -__builtin_inff();
+#pragma unroll
+                        for (int e = 0; e < Z::VW; ++e) st.v[t][i][e] = seen ? st.v[t][i][e] : 0u;   // 0 * NaN of a stale row is NaN
+                    }
+            }
+            float mx = x[0][0];
+#pragma unroll
+            for (int t = 0; t < SUB; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mx = fmaxf(mx, x[t][i]);
+            if (__any(mx > m + (kRaise + kBias))) {
+                const float mn = fmaxf(m, max_over_groups(mx) - kBias);
+                const float corr = __builtin_amdgcn_exp2f(m - mn);
+                m = mn;
+                l *= corr;
+#pragma unroll
+                for (int n = 0; n < Z::NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[n][i] *= corr;
+            }
+#pragma unroll
+            for (int t = 0; t < SUB; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[t][i] = __builtin_amdgcn_exp2f(x[t][i] - m);
+                    l += x[t][i];
+                }
+            if constexpr (DT == kF32) {
+#pragma unroll
+                for (int t = 0; t < SUB; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int n = 0; n < Z::NT; ++n)
+                            acc[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, st.v[t][i][n]), x[t][i], acc[n], 0, 0, 0);
+            } else {
+                uint32_t p[SUB][2];
+#pragma unroll
+                for (int t = 0; t < SUB; ++t)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t hi = __builtin_bit_cast(uint32_t, half2_t{(_Float16)x[t][2 * i], (_Float16)x[t][2 * i + 1]});
+                        const uint32_t lo = pack_f16_remainder(x[t][2 * i], x[t][2 * i + 1], hi);
+                        p[t][i] = is_lo ? lo : hi;
+                    }
+                // dword e of a key's V piece against the same dword of its neighbour: columns side by side -> keys side by side
+                auto turned = [&](int t, int n, int pair) -> uint32_t {   // V^T operand dword: keys 2 pair, 2 pair + 1 of tile t, d-tile n
+                    const uint32_t* const ka = st.v[t][2 * pair];
+                    const uint32_t* const kb2 = st.v[t][2 * pair + 1];
+                    if constexpr (DT == kF16) {
+                        return __builtin_amdgcn_perm(kb2[n / 2], ka[n / 2], n % 2 ? 0x07060302u : 0x05040100u);
+                    } else {
+                        const uint32_t c = __builtin_amdgcn_perm(kb2[n / 4], ka[n / 4], n % 4 >= 2 ? 0x07030602u : 0x05010400u);
+                        const half2_t h = n % 2 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)c, 1.0f, true)
+                                                : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)c, 1.0f, false);
+                        return __builtin_bit_cast(uint32_t, h);
+                    }
+                };
+                if constexpr (SUB % 2 == 0) {
+#pragma unroll
+                    for (int t = 0; t < SUB; t += 2) {
+                        const half8_t pb = __builtin_bit_cast(half8_t, u32x4{p[t][0], p[t][1], p[t + 1][0], p[t + 1][1]});
+#pragma unroll
+                        for (int n = 0; n < Z::NT; ++n) {
+                            const half8_t va = __builtin_bit_cast(half8_t, u32x4{turned(t, n, 0), turned(t, n, 1), turned(t + 1, n, 0), turned(t + 1, n, 1)});
+                            acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pb, acc[n], 0, 0, 0);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int t = 0; t < SUB; ++t) {
+                        const half4_t pb = __builtin_bit_cast(half4_t, u32x2{p[t][0], p[t][1]});
+#pragma unroll
+                        for (int n = 0; n < Z::NT; ++n) {
+                            const half4_t va = __builtin_bit_cast(half4_t, u32x2{turned(t, n, 0), turned(t, n, 1)});
+                            acc[n] = __builtin_amdgcn_mfma_f32_16x16x16f16(va, pb, acc[n], 0, 0, 0);
+                        }
+                    }
+                }
+            }
+        };
+
+        if (ua + (uint32_t)w < ub) {
+            Stage st0, st1;
+            uint32_t u = ua + (uint32_t)w;
+            Pages p0 = get_pages(u), p1 = get_pages(u + kDecWaves);
+            load(st0, p0, u);
+            for (;;) {
+                Pages p2 = get_pages(u + 2u * kDecWaves);
+                load(st1, p1, u + kDecWaves);
+                compute(st0, p0, u);
+                u += kDecWaves;
+                if (u >= ub) break;
+                p0 = p2;
+                p2 = get_pages(u + 2u * kDecWaves);
+                load(st0, p0, u + kDecWaves);
+                compute(st1, p1, u);
+                u += kDecWaves;
+                if (u >= ub) break;
+                p1 = p2;
+            }
+        }
+
+        // ---- the four wavefronts' parts joined through LDS
+        l = sum_over_groups(l);
+        if constexpr (DT != kF32) {
+#pragma unroll
+            for (int n = 0; n < Z::NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[n][i] = ror8_sum(acc[n][i]);
+        }
+        if (!is_lo) {
+#pragma unroll
+            for (int y = 0; y < Z::VP; ++y)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < Z::PE; j += 4) {
+                        float4_t v;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] = acc[y * Z::PE + j + e][i];
+                        *reinterpret_cast<float4_t*>(&o_lds[w][col][(16 * y + 4 * g + i) * Z::PE + j]) = v;
+                    }
+            if (g == 0) { m_lds[w][col] = m; l_lds[w][col] = l; }
+        }
+        __syncthreads();
+        const bool whole = ua == 0u && ub == pe - ps;
+        const uint64_t part = (uint64_t)wg * 2u + (s == s_first ? 0u : 1u);
+        for (uint32_t e = tid; e < heads * (D / 4); e += 256u) {
+            const uint32_t h = e / (D / 4), d = (e % (D / 4)) * 4u;
+            float M = m_lds[0][h];
+#pragma unroll
+            for (int i = 1; i < kDecWaves; ++i) M = fmaxf(M, m_lds[i][h]);
+            float L = 0.f;
+            float4_t sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < kDecWaves; ++i) {
+                const float f = __builtin_amdgcn_exp2f(m_lds[i][h] - M);
+                L = __builtin_fmaf(l_lds[i][h], f, L);
+                const float4_t v = *reinterpret_cast<const float4_t*>(&o_lds[i][h][d]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sum[j] = __builtin_fmaf(v[j], f, sum[j]);
+            }
+            if (d < dr) {
+                if (whole) {
+                    const float inv = L != 0.f ? 1.0f / L : 0.f;
+                    const uint64_t at = (uint64_t)s * a.o_stride + (uint64_t)(h0 + h) * dr + d;
+                    if (a.io_f16) {
+                        half4_t r;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) r[j] = (_Float16)(sum[j] * inv);
+                        *reinterpret_cast<half4_t*>(reinterpret_cast<_Float16*>(a.o) + at) = r;
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) sum[j] *= inv;
+                        *reinterpret_cast<float4_t*>(reinterpret_cast<float*>(a.o) + at) = sum;
+                    }
+                } else {
+                    const uint64_t row = part * a.n_heads + h0 + h;
+                    *reinterpret_cast<float4_t*>(a.scratch_out + row * dr + d) = sum;
+                    if (d == 0u) { a.scratch_max[row] = M; a.scratch_sum[row] = L; }
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// Joins the parts of the sequences that lie in more than one workgroup's range: one workgroup per (head, sequence).  The parts are
+// dealt to groups of D / 4 threads, each thread four columns.
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnLaunch a, uint32_t n_wg, uint32_t uk) {
+    __shared__ uint32_t red[2][kDecWaves];
+    __shared__ float4_t sums[256];
+    __shared__ float ls[256];
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const uint32_t head = blockIdx.x, s = blockIdx.y;
+    const uint32_t mine = seq_units(paged_kv_len(a.s, s), a.window, a.n_sink, uk).units;
+    uint32_t before = 0u, all = 0u;
+    for (uint32_t t = tid; t < a.s.n_seqs; t += 256u) {
+        const uint32_t x = seq_units(paged_kv_len(a.s, t), a.window, a.n_sink, uk).units;
+        all += x;
+        before += t < s ? x : 0u;
+    }
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) {
+        before += __shfl_xor(before, off, kWave);
+        all += __shfl_xor(all, off, kWave);
+    }
+    if (lane == 0) { red[0][w] = before; red[1][w] = all; }
+    __syncthreads();
+    before = red[0][0] + red[0][1] + red[0][2] + red[0][3];
+    const uint32_t U = red[1][0] + red[1][1] + red[1][2] + red[1][3];
+    if (mine == 0u) return;
+    // workgroup of unit u: the largest w with w U / N <= u
+    n_wg = used_wgs(U, n_wg);
+    const uint32_t wa = (uint32_t)((((uint64_t)before + 1u) * n_wg - 1u) / U);
+    const uint32_t wb = (uint32_t)((((uint64_t)before + mine) * n_wg - 1u) / U);
+    if (wa == wb) return;                                                // written by the workgroup itself
+    const uint32_t dr = a.c.head_dim, quads = dr / 4u;
+    const uint32_t groups = 256u / quads, grp = (uint32_t)tid / quads, q4 = (uint32_t)tid % quads;
+    auto part_row = [&](uint32_t x) {
+        const bool first = (uint64_t)x * U / n_wg >= before;             // the sequence is the first of that range
+        return ((uint64_t)x * 2u + (first ? 0u : 1u)) * a.n_heads + head;
+    };
+    float M = kMasked;
+    for (uint32_t x = wa + (uint32_t)lane; x <= wb; x += 64u) M = fmaxf(M, a.scratch_max[part_row(x)]);
+    M = wave_max_all(M);
+    float4_t sum = {0.f, 0.f, 0.f, 0.f};
+    float L = 0.f;
+    if (grp < groups) {
+        for (uint32_t x = wa + grp; x <= wb; x += groups) {
+            const uint64_t row = part_row(x);
+            const float f = __builtin_amdgcn_exp2f(a.scratch_max[row] - M);
+            const float4_t v = *reinterpret_cast<const float4_t*>(a.scratch_out + row * dr + q4 * 4u);
+            L = __builtin_fmaf(a.scratch_sum[row], f, L);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sum[j] = __builtin_fmaf(v[j], f, sum[j]);
+        }
+    }
+    sums[tid] = sum;
+    ls[tid] = L;
+    __syncthreads();
+    if (grp != 0u) return;
+    for (uint32_t x = 1; x < groups; ++x) {
+        const float4_t v = sums[x * quads + q4];
+        L += ls[x * quads + q4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[j] += v[j];
+    }
+    const float inv = L != 0.f ? 1.0f / L : 0.f;
+    const uint64_t at = (uint64_t)s * a.o_stride + (uint64_t)head * dr + q4 * 4u;
+    if (a.io_f16) {
+        half4_t r;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r[j] = (_Float16)(sum[j] * inv);
+        *reinterpret_cast<half4_t*>(reinterpret_cast<_Float16*>(a.o) + at) = r;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[j] *= inv;
+        *reinterpret_cast<float4_t*>(reinterpret_cast<float*>(a.o) + at) = sum;
+    }
+}
+
+uint32_t paged_decode_wgs(uint32_t head_groups) { return (512u + head_groups - 1u) / head_groups; }
+
+namespace {
+
+template <int DT, int D, int SUB>
+hipError_t launch_dec(const PagedAttnLaunch& L, hipStream_t stream) {
+    constexpr uint32_t UK = 16u * SUB;
+    const uint32_t slices = (L.n_heads / L.c.n_kv_heads + kDecHeads - 1u) / kDecHeads;
+    const uint32_t n_hg = L.c.n_kv_heads * slices;
+    // an upper bound of the units from what the host knows
+    uint64_t keys = L.max_kv;
+    if (L.window != 0u && (uint64_t)L.window + L.n_sink + 2u * UK < keys) keys = (uint64_t)L.window + L.n_sink + 2u * UK;
+    const uint64_t units = (uint64_t)L.s.n_seqs * ((keys + UK - 1u) / UK);
+    uint64_t n = paged_decode_wgs(n_hg);
+    const uint64_t useful = (units + 2u * kDecWaves - 1u) / (2u * kDecWaves);   // at least two units per wavefront
+    if (n > useful) n = useful;
+    const uint64_t fits = L.scratch_rows / (2u * (uint64_t)L.n_heads);
+    if (n > fits) n = fits;
+    if (n == 0u) n = 1u;
+    hipLaunchKernelGGL((paged_decode_kernel<DT, D, SUB>), dim3(n_hg, (uint32_t)n), dim3(256), (L.s.n_seqs + 1u) * 4u, stream, L, (uint32_t)n, slices);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || n == 1u) return e;
+    hipLaunchKernelGGL(paged_merge_kernel, dim3(L.n_heads, L.s.n_seqs), dim3(256), 0, stream, L, (uint32_t)n, UK);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_paged_decode(const PagedAttnLaunch& L, hipStream_t stream) {
+    const uint32_t d = L.c.head_dim;
+    if (L.c.dtype == kF8) {
+        if (d <= 64u) return launch_dec<kF8, 64, 4>(L, stream);
+        if (d <= 128u) return launch_dec<kF8, 128, 2>(L, stream);
+        return launch_dec<kF8, 256, 2>(L, stream);
+    }
+    if (L.c.dtype == kF16) {
+        if (d <= 64u) return launch_dec<kF16, 64, 2>(L, stream);
+        if (d <= 128u) return launch_dec<kF16, 128, 2>(L, stream);
+        return launch_dec<kF16, 256, 1>(L, stream);
+    }
+    if (d <= 64u) return launch_dec<kF32, 64, 1>(L, stream);
+    if (d <= 128u) return launch_dec<kF32, 128, 1>(L, stream);
+    return launch_dec<kF32, 256, 1>(L, stream);
+}
+
+}  // namespace vfkv
