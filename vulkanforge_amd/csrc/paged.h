@@ -62,9 +62,9 @@ struct PagedCopyLaunch {
 
 hipError_t launch_paged_copy(const PagedCopyLaunch& L, hipStream_t stream);
 hipError_t launch_paged_write(const PagedWriteLaunch& L, hipStream_t stream);
-// Matrix-core kernels: head_dim a multiple of 16 up to 256; q and o 16-byte aligned with strides that keep every row so
-// (paged_rows_aligned).
+// Matrix-core kernels: head_dim a multiple of 16 up to 256; q and o 16-byte aligned with strides that keep every row so.
 hipError_t launch_paged_decode(const PagedAttnLaunch& L, hipStream_t stream);
+hipError_t launch_paged_prefill(const PagedAttnLaunch& L, hipStream_t stream);
 // Workgroups per head group (KV head and slice of its query heads) the decode launch may use: its scratch holds two partial
 // rows per workgroup and head.
 uint32_t paged_decode_wgs(uint32_t head_groups);

@@ -460,6 +460,7 @@ static int paged_attention(vfkv_pages* c, uint32_t layer, const vfkv_seq_batch* 
     if (q == o) return fail(VFKV_ERR_INVALID_ARG, "%s: o must not overlap q", who);
     if ((((uintptr_t)q | (uintptr_t)o) & (p->io_dtype == VFKV_F32 ? 3u : 1u)) != 0u)
         return fail(VFKV_ERR_ALIGNMENT, "%s: a buffer is not aligned to its element size", who);
+    if ((uint64_t)b->n_tokens * p->n_heads > 0xFFFFFFFFull) return fail(VFKV_ERR_OVERFLOW, "%s: n_tokens * n_heads exceeds 2^32 - 1", who);
     if (ws && (ws->n_heads < p->n_heads || ws->head_dim < hd))
         return fail(VFKV_ERR_WORKSPACE, "%s: workspace built for %u heads x %u dims, need %u x %u", who, ws->n_heads, ws->head_dim, p->n_heads, hd);
     if (decode && !ws) return fail(VFKV_ERR_INVALID_ARG, "%s: workspace is NULL", who);
@@ -477,12 +478,12 @@ static int paged_attention(vfkv_pages* c, uint32_t layer, const vfkv_seq_batch* 
     vfkv::clear_note();
     const uint32_t per16 = p->io_dtype == VFKV_F32 ? 4u : 8u;
     const bool aligned = (((uintptr_t)q | (uintptr_t)o) & 15u) == 0u && L.q_stride % per16 == 0u && L.o_stride % per16 == 0u;
-    if (hd % 16u != 0u || hd > 256u || !aligned || !decode) {
+    if (hd % 16u != 0u || hd > 256u || !aligned) {
         VFKV_HIP(vfkv::launch_paged_generic(L, S(stream)));
         vfkv::note_generic(who, c->cfg.dtype, hd);
         return VFKV_OK;
     }
-    VFKV_HIP(vfkv::launch_paged_decode(L, S(stream)));
+    VFKV_HIP(decode ? vfkv::launch_paged_decode(L, S(stream)) : vfkv::launch_paged_prefill(L, S(stream)));
     return VFKV_OK;
 }
 
