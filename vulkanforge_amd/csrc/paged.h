@@ -65,6 +65,10 @@ hipError_t launch_paged_write(const PagedWriteLaunch& L, hipStream_t stream);
 // Matrix-core kernels: head_dim a multiple of 16 up to 256; q and o 16-byte aligned with strides that keep every row so.
 hipError_t launch_paged_decode(const PagedAttnLaunch& L, hipStream_t stream);
 hipError_t launch_paged_prefill(const PagedAttnLaunch& L, hipStream_t stream);
+hipError_t launch_paged_prefill_full(const PagedAttnLaunch& L, hipStream_t stream);    // F32 pages
+hipError_t launch_paged_prefill_half(const PagedAttnLaunch& L, hipStream_t stream);    // F16
+hipError_t launch_paged_prefill_byte(const PagedAttnLaunch& L, hipStream_t stream);    // FP8
+hipError_t launch_paged_rows_merge(const PagedAttnLaunch& L, uint32_t n_split, hipStream_t stream);
 // Workgroups per head group (KV head and slice of its query heads) the decode launch may use: its scratch holds two partial
 // rows per workgroup and head.
 uint32_t paged_decode_wgs(uint32_t head_groups);

@@ -1,0 +1,623 @@
+// Prefill attention over the paged cache: a ragged batch of chunks, causal, with a window per query and first tokens kept.
+//
+// o[r] = sum_j softmax_j(scale q[r].k_j) v_j over the keys row r sees; 4 * head_dim flop per visible (query row, key) pair, so
+// for chunks of any length the matrix cores bound it.
+//
+//   - The query heads of one KV head and the tokens of a chunk form one line of rows (token major): a workgroup takes a block of
+//     R = 128 NQ consecutive rows of one sequence and one KV head, a wavefront 32 NQ of them.  K and V are shared by the whole
+//     group, and short chunks (drafted tokens) fill the tiles with heads.  Blocks are numbered by a prefix sum over the
+//     batch that every workgroup forms itself (the offsets are device data), the last block of a sequence first: it has the most keys.
+//   - Keys pass through LDS in tiles of KT, as f16 (or f32), once for all rows of the workgroup: global loads of tile t + 1 run
+//     during the products of tile t, two LDS buffers, one barrier per tile.  A 16-key tile lies in one page, whose number is a
+//     scalar load two tiles ahead.
+//   - S^T = K Q^T and O^T += V^T P^T on v_mfma_f32_32x32x16_f16: the scores of a row stay in one lane and its opposite half, P is
+//     already where the second product wants it, V^T comes from the transposing LDS read.
+//   - f16 queries enter as they are and the weights as f16 (half a step of 2^-11 per weight, like the output's own rounding).  f32
+//     queries enter as f16 value + remainder, and so do the weights: f32-level accuracy for twice the products.
+//     F32 caches use the f32 matrix instruction.
+//   - The running maximum is only raised when a score exceeds it by 2^8; weights are kept times 2^6 (see paged_decode.hip).
+//   - Few rows over many keys: the tiles are cut into n_split parts over more workgroups and joined by paged_rows_merge_kernel.
+#pragma once
+#include <type_traits>
+
+#include "device_utils.h"
+#include "paged.h"
+
+namespace vfkv {
+
+namespace {
+
+constexpr float kRaise = 8.f, kBias = 6.f;  // log2
+
+template <int DT, int D, int KT, int NW>
+struct PreShape {
+    static constexpr int ES = DT == kF32 ? 4 : DT == kF16 ? 2 : 1;
+    static constexpr int LE = DT == kF32 ? 4 : 2;              // bytes per element in LDS
+    static constexpr int CPR = D * ES / 16;                    // 16-byte chunks per cache row
+    static constexpr int RPP = NW * 64 / CPR;                      // rows per staging pass
+    static constexpr int NP = KT / RPP;                        // passes per tile and tensor
+    // pitches: 16-byte reads of eight K rows, and reads of four (f16) / two (f32, four rows apart) V rows, hit distinct banks
+    static constexpr int KPITCH = D * LE + 16;                 // bytes
+    static constexpr int VPITCH = D * LE + (DT == kF32 ? 32 : 64);
+    static constexpr int BUF = KT * (KPITCH + VPITCH);         // one buffer: K tile, V tile
+    static_assert(KT % RPP == 0 || RPP > KT, "whole passes");
+};
+
+// Elements of a dword of the cache that are infinite or NaN, as a mask of their bits.
+template <int DT>
+__device__ __forceinline__ uint32_t not_finite(uint32_t x) {
+    if constexpr (DT == kF32) return (x & 0x7F800000u) == 0x7F800000u ? 0xFFFFFFFFu : 0u;
+    if constexpr (DT == kF16) return ((x & 0x7C00u) == 0x7C00u ? 0xFFFFu : 0u) | ((x & 0x7C000000u) == 0x7C000000u ? 0xFFFF0000u : 0u);
+    const uint32_t top = ((x & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;        // E4M3FN: only codes 0x7F and 0xFF
+    return top | (top - (top >> 7));
+}
+
+__device__ __forceinline__ float max_over_halves(float x) {
+    float y = x;
+    swap32(x, y);
+    return fmaxf(x, y);
+}
+
+}  // namespace
+
+// Exclusive prefix sums of the row blocks of the sequences, by the whole workgroup.
+template <int NW>
+__device__ __forceinline__ void block_prefix(const PagedAttnLaunch& a, uint32_t group, uint32_t rows, uint32_t* pre, uint32_t* wave_sum, int tid) {
+    const int lane = tid & 63, w = tid >> 6;
+    uint32_t carry = 0u;
+    for (uint32_t base = 0; base < a.s.n_seqs; base += NW * 64u) {
+        const uint32_t s = base + (uint32_t)tid;
+        uint32_t x = 0u;
+        if (s < a.s.n_seqs) {
+            uint32_t lo, hi;
+            paged_rows(a.s, s, lo, hi);
+            x = (uint32_t)(((uint64_t)(hi - lo) * group + rows - 1u) / rows);
+        }
+        const uint32_t mine = x;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const uint32_t y = __shfl_up(x, off, kWave);
+            if (lane >= off) x += y;
+        }
+        if (lane == 63) wave_sum[w] = x;
+        __syncthreads();
+        uint32_t before = carry;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+            if (i < w) before += wave_sum[i];
+            carry += wave_sum[i];
+        }
+        if (s < a.s.n_seqs) pre[s] = before + x - mine;
+        __syncthreads();
+    }
+    if (tid == 0) pre[a.s.n_seqs] = carry;
+    __syncthreads();
+}
+
+template <int DT, int D, bool IOF16, bool CAP, int NQ, int KT, int NW, int MINW>
+__global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnLaunch a, uint32_t n_split) {
+    using Z = PreShape<DT, D, KT, NW>;
+    constexpr bool F32C = DT == kF32;
+    constexpr bool PAIR = !IOF16 && !F32C;                   // queries and weights as value + remainder
+    constexpr int NB = KT / 32;                              // 32-key blocks per tile
+    constexpr int DT32 = D / 32;
+    constexpr uint32_t R = 32u * NQ * NW;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];   // two buffers, then the prefix sums
+    __shared__ uint32_t wave_sum[NW];
+    // keys whose V row holds an infinity or NaN, from tiles that are hidden in part: at most the tiles the block's queries and
+    // the two ends of its window cut through
+    constexpr uint32_t kOddMax = KT * (2u * (R / KT + 2u) + 1u);
+    __shared__ uint32_t n_odd, odd_key[kOddMax];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n32 = lane & 31, hf = lane >> 5;
+    const uint32_t group = a.n_heads / a.c.n_kv_heads, kvh = blockIdx.x;
+    const uint32_t dr = a.c.head_dim;
+    uint32_t* const pre = reinterpret_cast<uint32_t*>(lds + 2 * Z::BUF);
+    if (tid == 0) n_odd = 0u;
+    block_prefix<NW>(a, group, R, pre, wave_sum, tid);
+    const uint32_t blocks = __builtin_amdgcn_readfirstlane(pre[a.s.n_seqs]);
+    if (blockIdx.y >= blocks) return;
+    const uint32_t bi = blocks - 1u - blockIdx.y;
+    uint32_t s;
+    {
+        uint32_t x = 0u, y = a.s.n_seqs - 1u;                // the last s with pre[s] <= bi
+        while (x < y) {
+            const uint32_t mid = (x + y + 1u) >> 1;
+            if (pre[mid] <= bi) x = mid; else y = mid - 1u;
+        }
+        s = __builtin_amdgcn_readfirstlane(x);
+    }
+    uint32_t t0, t1;
+    paged_rows(a.s, s, t0, t1);
+    t0 = __builtin_amdgcn_readfirstlane(t0);
+    t1 = __builtin_amdgcn_readfirstlane(t1);
+    const uint32_t n_rows = (t1 - t0) * group;               // (< 2^31 * 2^16 would not fit: the launcher refuses n_tokens * n_heads >= 2^32)
+    const uint32_t row0 = (bi - __builtin_amdgcn_readfirstlane(pre[s])) * R;
+    const uint32_t row1 = n_rows - row0 < R ? n_rows : row0 + R;
+    const int kv_len = (int)__builtin_amdgcn_readfirstlane(paged_kv_len(a.s, s));
+    const int pos0 = kv_len - (int)(t1 - t0);                // position of the chunk's first token
+    const int pmin = pos0 + (int)(row0 / group), pmax = pos0 + (int)((row1 - 1u) / group);
+    // key tiles of the block: first tokens in front of the window of its first query, then up to its last query
+    const uint32_t n_keys = pmax < 0 ? 0u : (uint32_t)pmax + 1u;
+    const uint32_t lo_min = pmin > 0 ? paged_window_lo(a.window, (uint32_t)pmin) : 0u;
+    const uint32_t first = lo_min / KT;
+    const uint32_t sink = a.n_sink < lo_min ? a.n_sink : lo_min;
+    const uint32_t su = (sink + KT - 1u) / KT;
+    const uint32_t sink_tiles = su < first ? su : first;
+    const uint32_t tiles = n_keys ? sink_tiles + (n_keys + KT - 1u) / KT - first : 0u;
+    const uint32_t ta = (uint32_t)((uint64_t)blockIdx.z * tiles / n_split), tb = (uint32_t)((uint64_t)(blockIdx.z + 1u) * tiles / n_split);
+    auto tile_key = [&](uint32_t t) { return (t < sink_tiles ? t : first + t - sink_tiles) * (uint32_t)KT; };
+
+    // ---- this wavefront's rows
+    const uint32_t wr0 = row0 + (uint32_t)w * 32u * NQ;
+    const bool wave_has = wr0 < row1;
+    const uint32_t wr1 = row1 < wr0 + 32u * NQ ? row1 : wr0 + 32u * NQ;
+    const int wmin = wave_has ? pos0 + (int)(wr0 / group) : 0, wmax = wave_has ? pos0 + (int)((wr1 - 1u) / group) : -1;
+    const int wlo_max = wmax > 0 ? (int)paged_window_lo(a.window, (uint32_t)wmax) : 0;     // window start of the last query
+    const int wlo_min = wmin > 0 ? (int)paged_window_lo(a.window, (uint32_t)wmin) : 0;
+    uint32_t lo[NQ], span[NQ], lead[NQ];                     // a row sees the keys [lo, lo + span) and [0, lead)
+    uint32_t tok[NQ], head[NQ];
+    bool real[NQ];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+        const uint32_t r = wr0 + 32u * q + (uint32_t)n32;
+        real[q] = r < row1;
+        const uint32_t rr = real[q] ? r : row0;
+        tok[q] = rr / group;
+        head[q] = kvh * group + rr - tok[q] * group;
+        const int pos = real[q] ? pos0 + (int)tok[q] : -1;
+        lo[q] = pos > 0 ? paged_window_lo(a.window, (uint32_t)pos) : 0u;
+        span[q] = pos < 0 ? 0u : (uint32_t)pos + 1u - lo[q];
+        lead[q] = pos < 0 ? 0u : a.n_sink < (uint32_t)pos + 1u ? a.n_sink : (uint32_t)pos + 1u;
+        tok[q] += t0;
+    }
+    // ---- Q^T operands
+    half8_t qh[F32C ? 1 : NQ][F32C ? 1 : D / 16], ql[PAIR ? NQ : 1][PAIR ? D / 16 : 1];
+    float qf[F32C ? NQ : 1][F32C ? D / 2 : 1];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+        const uint64_t at = (uint64_t)tok[q] * a.q_stride + (uint64_t)head[q] * dr;
+        if constexpr (F32C) {
+#pragma unroll
+            for (int c = 0; c < D / 8; ++c) {
+                const uint32_t d = 8u * c + 4u * (uint32_t)hf;
+                const bool ok = real[q] && d < dr;
+                float4_t x;
+                if constexpr (IOF16) {
+                    const half4_t h = *reinterpret_cast<const half4_t*>(reinterpret_cast<const _Float16*>(a.q) + at + (ok ? d : 0u));
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x[j] = (float)h[j];
+                } else {
+                    x = *reinterpret_cast<const float4_t*>(reinterpret_cast<const float*>(a.q) + at + (ok ? d : 0u));
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) qf[q][4 * c + j] = ok ? x[j] : 0.f;
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) {
+                const uint32_t d = 16u * c + 8u * (uint32_t)hf;
+                const bool ok = real[q] && d < dr;
+                if constexpr (IOF16) {
+                    const half8_t x = *reinterpret_cast<const half8_t*>(reinterpret_cast<const _Float16*>(a.q) + at + (ok ? d : 0u));
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) qh[q][c][j] = ok ? x[j] : (_Float16)0.f;
+                } else {
+                    const float* const src = reinterpret_cast<const float*>(a.q) + at + (ok ? d : 0u);
+                    const float4_t x0 = *reinterpret_cast<const float4_t*>(src), x1 = *reinterpret_cast<const float4_t*>(src + 4);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float x = ok ? (j < 4 ? x0[j & 3] : x1[j & 3]) : 0.f;
+                        const _Float16 hi = (_Float16)x;
+                        qh[q][c][j] = hi;
+                        ql[q][c][j] = (_Float16)(x - (float)hi);
+                    }
+                }
+            }
+        }
+    }
+
+    float16_t acc[DT32][NQ];
+    float m[NQ], l[NQ];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+        m[q] = kMasked;
+        l[q] = 0.f;
+#pragma unroll
+        for (int n = 0; n < DT32; ++n)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[n][q][e] = 0.f;
+    }
+    const float scale_l2 = a.scale * 1.44269504088896f;
+    const float cap_l2 = a.softcap * 1.44269504088896f;
+    const float inv_cap_l2 = CAP ? 1.0f / cap_l2 : 0.f;
+    const float fac = CAP ? 1.0f : scale_l2;                 // scores are kept unscaled; the soft-cap leaves them in log2 units
+
+    // ---- staging
+    const uint32_t row_b = dr * Z::ES;
+    const uint32_t chunk = (uint32_t)tid % Z::CPR, srow = (uint32_t)tid / Z::CPR;
+    const bool chunk_ok = chunk * 16u < row_b;
+    const uint64_t head_rows = (uint64_t)kvh << a.c.page_shift;
+    const uint32_t slot_mask = (1u << a.c.page_shift) - 1u;
+    const int32_t* const table = a.s.table + (uint64_t)s * a.s.table_stride;
+    constexpr int NP = Z::NP < 1 ? 1 : Z::NP;
+    constexpr int SUBS = KT / 16;                            // 16-key tiles: each lies in one page
+    struct Pages {
+        uint32_t tile[SUBS];                                 // pages of the tile, for masking
+        uint32_t pass[NP];                                   // pages of the rows this wavefront stages (one page per wavefront and pass)
+    };
+    const uint32_t wave_row = (uint32_t)w * (64u / Z::CPR);
+    auto page_at = [&](uint32_t key) { return (uint32_t)table[(key < n_keys ? key : n_keys - 1u) >> a.c.page_shift]; };
+    auto get_pages = [&](uint32_t t) {
+        Pages r;
+        const uint32_t kb = tile_key(t < tb ? t : tb - 1u);
+#pragma unroll
+        for (int i = 0; i < SUBS; ++i) r.tile[i] = page_at(kb + 16u * i);
+#pragma unroll
+        for (int p = 0; p < NP; ++p) r.pass[p] = page_at(kb + (((uint32_t)(p * Z::RPP) + wave_row) & (KT - 16u)));
+        return r;
+    };
+    u32x4 kraw[NP], vraw[NP];
+    auto fetch = [&](const Pages& P, uint32_t t) {
+        const uint32_t kb = tile_key(t);
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            const uint32_t page = P.pass[p] < a.c.n_pages ? P.pass[p] : 0u;
+            const uint32_t key = kb + (((uint32_t)(p * Z::RPP) + wave_row) & (KT - 16u));
+            const uint64_t off = (uint64_t)page * a.c.page_bytes + (head_rows + (key & slot_mask)) * row_b;
+            const uint32_t lane_off = (((uint32_t)(p * Z::RPP) + srow) & 15u) * row_b + (chunk_ok ? chunk * 16u : 0u);
+            kraw[p] = *reinterpret_cast<const u32x4*>(a.c.k + off + lane_off);
+            vraw[p] = *reinterpret_cast<const u32x4*>(a.c.v + off + lane_off);
+        }
+    };
+    // In a tile that some query of the block does not see completely, V rows no query sees become zeros (their weights are zero, but
+    // 0 * NaN of a stale row is not), and so does every element that is not finite: queries the key is hidden from
+    // must not meet it.  The key is noted and the queries that do see it get the element when the output is written.
+    auto stage = [&](int buf, const Pages& P, uint32_t t) {
+        uint8_t* const kl = lds + buf * Z::BUF;
+        uint8_t* const vl = kl + KT * Z::KPITCH;
+        const uint32_t kb = tile_key(t);
+        const bool hidden = kb + KT > (uint32_t)(pmin < 0 ? 0 : pmin + 1) ||
+                            !(kb + KT <= a.n_sink || a.window == 0u || kb >= paged_window_lo(a.window, (uint32_t)pmax));
+        bool part = hidden;
+#pragma unroll
+        for (int i = 0; i < SUBS; ++i) part = part || P.tile[i] >= a.c.n_pages;
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            const uint32_t row = (uint32_t)(p * Z::RPP) + srow;
+            u32x4 k = kraw[p], v = vraw[p];
+            if (part) {
+                const uint32_t key = kb + row;
+                const bool ok = chunk_ok && key < n_keys && (key >= lo_min || key < sink) && P.pass[p] < a.c.n_pages;
+                bool odd = false;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t bad = not_finite<DT>(v[i]);
+                    odd = odd || (ok && bad != 0u);
+                    v[i] = ok ? (hidden ? v[i] & ~bad : v[i]) : 0u;
+                }
+                if (hidden && odd && row < (uint32_t)KT) {
+                    const uint64_t same = __ballot(odd) >> ((uint32_t)lane / Z::CPR * Z::CPR);   // (this lane's row: CPR lanes from there)
+                    if ((uint32_t)__builtin_ctzll(same) == (uint32_t)lane % Z::CPR) {
+                        const uint32_t at = atomicAdd(&n_odd, 1u);
+                        if (at < kOddMax) odd_key[at] = key;
+                    }
+                }
+            }
+            if (!chunk_ok) {
+                k = u32x4{0u, 0u, 0u, 0u};
+                v = k;
+            }
+            if (Z::RPP > KT && row >= (uint32_t)KT) continue;
+            if constexpr (DT == kF8) {
+                half2_t h[8];
+                u32x4 o[2];
+                auto widen = [&](const u32x4& x) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) e4m3x4_to_h2(x[i], h[2 * i], h[2 * i + 1]);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) o[i / 4][i % 4] = __builtin_bit_cast(uint32_t, h[i]);
+                };
+                widen(k);
+                *reinterpret_cast<u32x4*>(kl + row * Z::KPITCH + chunk * 32u) = o[0];
+                *reinterpret_cast<u32x4*>(kl + row * Z::KPITCH + chunk * 32u + 16u) = o[1];
+                widen(v);
+                *reinterpret_cast<u32x4*>(vl + row * Z::VPITCH + chunk * 32u) = o[0];
+                *reinterpret_cast<u32x4*>(vl + row * Z::VPITCH + chunk * 32u + 16u) = o[1];
+            } else {
+                *reinterpret_cast<u32x4*>(kl + row * Z::KPITCH + chunk * 16u) = k;
+                *reinterpret_cast<u32x4*>(vl + row * Z::VPITCH + chunk * 16u) = v;
+            }
+        }
+    };
+
+    // ---- one tile
+    auto compute = [&](auto masked, int buf, const Pages& P, uint32_t t) {
+        constexpr bool MASKED = decltype(masked)::value;     // some of the wavefront's queries do not see some of the keys
+        const uint8_t* const kl = lds + buf * Z::BUF;
+        const uint8_t* const vl = kl + KT * Z::KPITCH;
+        const int kb = (int)tile_key(t);
+        float16_t sc[NB][NQ];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+#pragma unroll
+            for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sc[b][q][e] = 0.f;
+            const uint8_t* const krow = kl + (32 * b + n32) * Z::KPITCH + hf * 16;
+            if constexpr (F32C) {
+#pragma unroll
+                for (int c = 0; c < D / 8; ++c) {
+                    const float4_t k = *reinterpret_cast<const float4_t*>(krow + 32 * c);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int q = 0; q < NQ; ++q) sc[b][q] = __builtin_amdgcn_mfma_f32_32x32x2f32(k[j], qf[q][4 * c + j], sc[b][q], 0, 0, 0);
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < D / 16; ++c) {
+                    const half8_t k = *reinterpret_cast<const half8_t*>(krow + 32 * c);
+#pragma unroll
+                    for (int q = 0; q < NQ; ++q) {
+                        sc[b][q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[q][c], sc[b][q], 0, 0, 0);
+                        if constexpr (PAIR) sc[b][q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[q][c], sc[b][q], 0, 0, 0);
+                    }
+                }
+            }
+        }
+        if constexpr (CAP) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) sc[b][q][e] = softcap_l2(sc[b][q][e] * scale_l2, cap_l2, inv_cap_l2);
+        }
+        if constexpr (MASKED) {
+            // key in [lo, pos] as one unsigned comparison against their number; a key among the first tokens as another
+            auto hide = [&](auto firsts) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const bool there = P.tile[2 * b + h] < a.c.n_pages;      // (uniform: 16 keys lie in one page)
+#pragma unroll
+                        for (int q = 0; q < NQ; ++q) {
+                            const uint32_t key = (uint32_t)(kb + 32 * b + 16 * h + 4 * hf), rel = key - lo[q];
+                            const uint32_t some = there ? span[q] : 0u, front = there ? lead[q] : 0u;
+#pragma unroll
+                            for (uint32_t x = 0; x < 8; ++x) {
+                                const uint32_t off = 8u * (x / 4u) + x % 4u;
+                                bool seen = rel + off < some;
+                                if constexpr (decltype(firsts)::value) seen = seen || key + off < front;
+                                sc[b][q][8 * h + x] = seen ? sc[b][q][8 * h + x] : -__builtin_inff();
+                            }
+                        }
+                    }
+            };
+            if ((uint32_t)kb < a.n_sink) hide(std::true_type{}); else hide(std::false_type{});
+        }
+        float mx[NQ];
+        bool raise = false;
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+            mx[q] = sc[0][q][0];
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) mx[q] = fmaxf(mx[q], sc[b][q][e]);
+            raise = raise || mx[q] * fac > m[q] + (kRaise + kBias);
+        }
+        if (__any(raise)) {
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) {
+                const float mn = fmaxf(m[q], max_over_halves(mx[q]) * fac - kBias);
+                const float corr = __builtin_amdgcn_exp2f(m[q] - mn);
+                m[q] = mn;
+                l[q] *= corr;
+#pragma unroll
+                for (int n = 0; n < DT32; ++n)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) acc[n][q][e] *= corr;
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    sc[b][q][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][q][e], fac, -m[q]));
+                    if constexpr (F32C || PAIR) l[q] += sc[b][q][e];
+                }
+        if constexpr (F32C) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const uint8_t* const vrow = vl + (32 * b + 8 * (e / 4) + 4 * hf + e % 4) * Z::VPITCH + n32 * 4;
+#pragma unroll
+                    for (int n = 0; n < DT32; ++n) {
+                        const float v = *reinterpret_cast<const float*>(vrow + 128 * n);
+#pragma unroll
+                        for (int q = 0; q < NQ; ++q) acc[n][q] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, sc[b][q][e], acc[n][q], 0, 0, 0);
+                    }
+                }
+        } else {
+            // lane's place in the transposing read: row 4 hf + (lane % 16) / 4 of eight-row steps, column group of its sixteen lanes
+            const uint8_t* const vlane = vl + (4 * hf + (lane & 15) / 4) * Z::VPITCH + (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
+#pragma unroll
+            for (int kk = 0; kk < KT / 16; ++kk) {
+                half8_t ph[NQ], pl[PAIR ? NQ : 1];
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) {
+                    uint32_t h[4], r[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float p0 = sc[kk / 2][q][8 * (kk % 2) + 2 * i], p1 = sc[kk / 2][q][8 * (kk % 2) + 2 * i + 1];
+                        const half2_t hh = half2_t{(_Float16)p0, (_Float16)p1};
+                        h[i] = __builtin_bit_cast(uint32_t, hh);
+                        // the sum of the weights as the product uses them: their rounding cancels in the mean
+                        if constexpr (!PAIR) l[q] = __builtin_amdgcn_fdot2(hh, half2_t{(_Float16)1.f, (_Float16)1.f}, l[q], false);
+                        if constexpr (PAIR) r[i] = pack_f16_remainder(p0, p1, h[i]);
+                    }
+                    ph[q] = __builtin_bit_cast(half8_t, h);
+                    if constexpr (PAIR) pl[q] = __builtin_bit_cast(half8_t, r);
+                }
+#pragma unroll
+                for (int n = 0; n < DT32; ++n) {
+                    const half4_t v0 = lds_read_tr16(reinterpret_cast<const _Float16*>(vlane + 16 * kk * Z::VPITCH + 64 * n));
+                    const half4_t v1 = lds_read_tr16(reinterpret_cast<const _Float16*>(vlane + (16 * kk + 8) * Z::VPITCH + 64 * n));
+                    const half8_t v = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+                    for (int q = 0; q < NQ; ++q) {
+                        acc[n][q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[q], acc[n][q], 0, 0, 0);
+                        if constexpr (PAIR) acc[n][q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[q], acc[n][q], 0, 0, 0);
+                    }
+                }
+            }
+        }
+    };
+
+    if (ta < tb) {
+        Pages p0 = get_pages(ta), p1 = get_pages(ta + 1u);
+        fetch(p0, ta);
+        stage(0, p0, ta);
+        for (uint32_t t = ta; t < tb; ++t) {
+            const int buf = (int)((t - ta) & 1u);
+            __syncthreads();                                   // tile t staged by all; tile t - 1 no longer read
+            const Pages p2 = get_pages(t + 2u);
+            if (t + 1u < tb) fetch(p1, t + 1u);
+            if (wave_has) {
+                const int kb = (int)tile_key(t);
+                bool ghost = false;
+#pragma unroll
+                for (int i = 0; i < SUBS; ++i) ghost = ghost || p0.tile[i] >= a.c.n_pages;
+                // (a tile that none of the wavefront's queries sees is passed over)
+                if (!(kb > wmax || ((uint32_t)kb >= a.n_sink && kb + KT <= wlo_min))) {
+                    if (kb + KT - 1 <= wmin && (kb >= wlo_max || (uint32_t)(kb + KT) <= a.n_sink) && !ghost) compute(std::false_type{}, buf, p0, t);
+                    else compute(std::true_type{}, buf, p0, t);
+                }
+            }
+            if (t + 1u < tb) stage(buf ^ 1, p1, t + 1u);
+            p0 = p1;
+            p1 = p2;
+        }
+    }
+
+    // ---- output
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+        const float L = xor32_sum(l[q]);
+        if (!real[q]) continue;
+        const float inv = n_split > 1u ? 1.0f : L != 0.f ? 1.0f / L : 0.f;
+        const uint64_t row = ((uint64_t)tok[q] * a.n_heads + head[q]) * n_split + blockIdx.z;
+        const uint64_t at = (uint64_t)tok[q] * a.o_stride + (uint64_t)head[q] * dr;
+        if (n_split > 1u && hf == 0) { a.scratch_max[row] = m[q]; a.scratch_sum[row] = L; }
+#pragma unroll
+        for (int n = 0; n < DT32; ++n)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const uint32_t d = 32u * n + 8u * b + 4u * (uint32_t)hf;
+                if (d >= dr) continue;
+                float4_t v;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = acc[n][q][4 * b + j] * inv;
+                if (n_split > 1u) {
+                    *reinterpret_cast<float4_t*>(a.scratch_out + row * dr + d) = v;
+                } else if constexpr (IOF16) {
+                    half4_t h;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) h[j] = (_Float16)v[j];
+                    *reinterpret_cast<half4_t*>(reinterpret_cast<_Float16*>(a.o) + at + d) = h;
+                } else {
+                    *reinterpret_cast<float4_t*>(reinterpret_cast<float*>(a.o) + at + d) = v;
+                }
+            }
+    }
+    // ---- noted keys: their infinities and NaNs go to the rows that see them, each lane on the elements it has just written
+    if (ta >= tb) return;
+    __syncthreads();                                         // the last tile's notes
+    const uint32_t n_bad = __builtin_amdgcn_readfirstlane(n_odd < kOddMax ? n_odd : kOddMax);
+#pragma unroll 1
+    for (uint32_t i = 0; i < n_bad; ++i) {
+        const uint32_t key = __builtin_amdgcn_readfirstlane(odd_key[i]);
+        const uint32_t page = (uint32_t)table[key >> a.c.page_shift];
+        const uint8_t* const vrow = a.c.v + (uint64_t)(page < a.c.n_pages ? page : 0u) * a.c.page_bytes + (head_rows + (key & slot_mask)) * row_b;
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+            if (!real[q] || !(key - lo[q] < span[q] || key < lead[q])) continue;
+            const uint64_t row = ((uint64_t)tok[q] * a.n_heads + head[q]) * n_split + blockIdx.z;
+            const uint64_t at = (uint64_t)tok[q] * a.o_stride + (uint64_t)head[q] * dr;
+#pragma unroll 1
+            for (uint32_t d = 4u * (uint32_t)hf; d < dr; d += 8u)
+#pragma unroll 1
+                for (uint32_t j = d; j < d + 4u; ++j) {
+                    const float v = load_kv_elem(vrow, DT, j);
+                    if (fabsf(v) < __builtin_inff()) continue;
+                    if (n_split > 1u) a.scratch_out[row * dr + j] += v;
+                    else if constexpr (IOF16) reinterpret_cast<_Float16*>(a.o)[at + j] = (_Float16)((float)reinterpret_cast<_Float16*>(a.o)[at + j] + v);
+                    else reinterpret_cast<float*>(a.o)[at + j] += v;
+                }
+        }
+    }
+}
+
+namespace {
+
+template <int DT, int D, bool IOF16, bool CAP, int NQ, int KT, int NW, int MINW>
+hipError_t launch_pre(const PagedAttnLaunch& L, hipStream_t stream) {
+    using Z = PreShape<DT, D, KT, NW>;
+    constexpr uint64_t R = 32u * NQ * NW;
+    const uint64_t group = L.n_heads / L.c.n_kv_heads;
+    // a sequence's last block may be ragged: at most one block more per sequence that has rows
+    const uint64_t with_rows = L.s.n_seqs < L.s.n_tokens ? L.s.n_seqs : L.s.n_tokens;
+    uint64_t blocks = L.s.n_tokens * group / R + with_rows;
+    if (blocks > L.s.n_tokens * group) blocks = L.s.n_tokens * group;
+    if (blocks > 65535u * 4096ull) return hipErrorInvalidValue;
+    // split over the keys: as long as the card has room, at least four tiles per part
+    const uint64_t likely = (L.s.n_tokens * group + R - 1u) / R * L.c.n_kv_heads;
+    const uint64_t room = 256u * MINW * 4u / NW;
+    uint64_t keys = L.max_kv;
+    if (L.window != 0u && (uint64_t)L.window + L.n_sink + R + 2u * KT < keys) keys = (uint64_t)L.window + L.n_sink + R + 2u * KT;
+    uint64_t n = room / likely;
+    if (n > keys / (4u * KT)) n = keys / (4u * KT);
+    const uint64_t fits = L.scratch_rows / ((uint64_t)L.s.n_tokens * L.n_heads);
+    if (n > fits) n = fits;
+    if (n > 64u) n = 64u;
+    if (n == 0u) n = 1u;
+    hipLaunchKernelGGL((paged_prefill_kernel<DT, D, IOF16, CAP, NQ, KT, NW, MINW>), dim3(L.c.n_kv_heads, (uint32_t)blocks, (uint32_t)n), dim3(NW * 64),
+                       2u * Z::BUF + (L.s.n_seqs + 1u) * 4u, stream, L, (uint32_t)n);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || n == 1u) return e;
+    return launch_paged_rows_merge(L, (uint32_t)n, stream);
+}
+
+template <int DT, bool IOF16, bool CAP>
+hipError_t launch_dim(const PagedAttnLaunch& L, hipStream_t stream) {
+    const uint32_t d = L.c.head_dim;
+    if constexpr (DT == kF32) {
+        if (d <= 64u) return launch_pre<DT, 64, IOF16, CAP, 1, 32, 4, 2>(L, stream);
+        if (d <= 128u) return launch_pre<DT, 128, IOF16, CAP, 1, 32, 4, 2>(L, stream);
+        return launch_pre<DT, 256, IOF16, CAP, 1, 32, 4, 1>(L, stream);
+    } else {
+        const bool many = (uint64_t)L.s.n_tokens * (L.n_heads / L.c.n_kv_heads) >= 256ull * L.s.n_seqs;
+        constexpr int KT = IOF16 ? 64 : 32;
+        if (d <= 64u) return many ? launch_pre<DT, 64, IOF16, CAP, 1, 64, 8, 2>(L, stream) : launch_pre<DT, 64, IOF16, CAP, 1, 64, 4, 2>(L, stream);
+        if (d <= 128u) return many ? launch_pre<DT, 128, IOF16, CAP, 1, KT, 8, 2>(L, stream) : launch_pre<DT, 128, IOF16, CAP, 1, KT, 4, 2>(L, stream);
+        return launch_pre<DT, 256, IOF16, CAP, 1, 32, 4, 1>(L, stream);
+    }
+}
+
+}  // namespace
+
+// One translation unit per cache type: paged_prefill_{full,half,byte}.hip.
+template <int DT>
+hipError_t launch_prefill_of(const PagedAttnLaunch& L, hipStream_t stream) {
+    if (L.softcap > 0.f) return L.io_f16 ? launch_dim<DT, true, true>(L, stream) : launch_dim<DT, false, true>(L, stream);
+    return L.io_f16 ? launch_dim<DT, true, false>(L, stream) : launch_dim<DT, false, false>(L, stream);
+}
+
+}  // namespace vfkv

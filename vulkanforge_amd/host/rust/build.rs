@@ -5,7 +5,8 @@ fn main() {
     let src = "vfkv/csrc";
     let mut objs = vec![];
     for f in ["api.hip", "kv_append.hip", "rope_append.hip", "gated_output.hip", "attn_decode.hip", "attn_prefill.hip",
-              "paged_api.hip", "paged_cache.hip", "paged_attn.hip", "paged_decode.hip", "paged_prefill.hip"] {
+              "paged_api.hip", "paged_cache.hip", "paged_attn.hip", "paged_decode.hip", "paged_prefill.hip", "paged_prefill_full.hip",
+              "paged_prefill_half.hip", "paged_prefill_byte.hip"] {
         let o = format!("{out}/{}.o", f.trim_end_matches(".hip"));
         let ok = Command::new("/opt/rocm/bin/hipcc")
             .args(["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
