@@ -305,11 +305,7 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
                     }
                 }
             }
-            if (!chunk_ok) {
-                k = u32x4{0u, 0u, 0u, 0u};
-                v = k;
-            }
-            if (Z::RPP > KT && row >= (uint32_t)KT) continue;
+            if (!chunk_ok || (Z::RPP > KT && row >= (uint32_t)KT)) continue;      // (columns past a narrower head stay zero)
             if constexpr (DT == kF8) {
                 half2_t h[8];
                 u32x4 o[2];
@@ -333,8 +329,7 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
     };
 
     // ---- one tile
-    auto compute = [&](auto masked, int buf, const Pages& P, uint32_t t) {
-        constexpr bool MASKED = decltype(masked)::value;     // some of the wavefront's queries do not see some of the keys
+    auto compute = [&](bool masked, int buf, const Pages& P, uint32_t t) {   // masked: some of the queries do not see some of the keys
         const uint8_t* const kl = lds + buf * Z::BUF;
         const uint8_t* const vl = kl + KT * Z::KPITCH;
         const int kb = (int)tile_key(t);
@@ -375,7 +370,7 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
 #pragma unroll
                     for (int e = 0; e < 16; ++e) sc[b][q][e] = softcap_l2(sc[b][q][e] * scale_l2, cap_l2, inv_cap_l2);
         }
-        if constexpr (MASKED) {
+        if (masked) {
             // key in [lo, pos] as one unsigned comparison against their number; a key among the first tokens as another
             auto hide = [&](auto firsts) {
 #pragma unroll
@@ -481,7 +476,10 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
         }
     };
 
+    if (dr < (uint32_t)D)                                    // columns past a narrower head: zeros in both buffers, for good
+        for (uint32_t i = (uint32_t)tid * 16u; i < 2u * Z::BUF; i += NW * 1024u) *reinterpret_cast<u32x4*>(lds + i) = u32x4{0u, 0u, 0u, 0u};
     if (ta < tb) {
+        if (dr < (uint32_t)D) __syncthreads();
         Pages p0 = get_pages(ta), p1 = get_pages(ta + 1u);
         fetch(p0, ta);
         stage(0, p0, ta);
@@ -496,10 +494,8 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
 #pragma unroll
                 for (int i = 0; i < SUBS; ++i) ghost = ghost || p0.tile[i] >= a.c.n_pages;
                 // (a tile that none of the wavefront's queries sees is passed over)
-                if (!(kb > wmax || ((uint32_t)kb >= a.n_sink && kb + KT <= wlo_min))) {
-                    if (kb + KT - 1 <= wmin && (kb >= wlo_max || (uint32_t)(kb + KT) <= a.n_sink) && !ghost) compute(std::false_type{}, buf, p0, t);
-                    else compute(std::true_type{}, buf, p0, t);
-                }
+                if (!(kb > wmax || ((uint32_t)kb >= a.n_sink && kb + KT <= wlo_min)))
+                    compute(!(kb + KT - 1 <= wmin && (kb >= wlo_max || (uint32_t)(kb + KT) <= a.n_sink) && !ghost), buf, p0, t);
             }
             if (t + 1u < tb) stage(buf ^ 1, p1, t + 1u);
             p0 = p1;
