@@ -9,6 +9,8 @@
 
 namespace vfkv {
 
+constexpr uint32_t kPagedMaxLen = 1u << 30;   // positions of one sequence: sums with a tile's keys stay in 31 bits
+
 struct PagedSlab {             // one layer
     const uint8_t* k;
     const uint8_t* v;
@@ -20,7 +22,7 @@ struct PagedSeqs {
     const int32_t* kv_lens;    // [n_seqs]
     const int32_t* q_offsets;  // [n_seqs + 1] or NULL: token t is the one token of sequence t
     uint32_t n_seqs, table_stride, n_tokens;
-    uint32_t limit;            // min(table_stride * page_size, 2^31 - 1)
+    uint32_t limit;            // min(table_stride * page_size, kPagedMaxLen): longest length the kernels follow
 };
 struct PagedAttnLaunch {
     PagedSlab c;

@@ -78,7 +78,7 @@ int check_batch(const vfkv_pages* c, const vfkv_seq_batch* b, const char* who, v
     const uint64_t held = (uint64_t)b->table_stride << c->page_shift;
     out->table = b->page_table; out->kv_lens = b->kv_lens; out->q_offsets = b->q_offsets;
     out->n_seqs = b->n_seqs; out->table_stride = b->table_stride; out->n_tokens = b->n_tokens;
-    out->limit = held < 0x7FFFFFFFu ? (uint32_t)held : 0x7FFFFFFFu;
+    out->limit = held < vfkv::kPagedMaxLen ? (uint32_t)held : vfkv::kPagedMaxLen;
     *max_kv = b->max_kv_len != 0u && b->max_kv_len < out->limit ? b->max_kv_len : out->limit;
     return VFKV_OK;
 }

@@ -4,7 +4,7 @@
 // for chunks of any length the matrix cores bound it.
 //
 //   - The query heads of one KV head and the tokens of a chunk form one line of rows (token major): a workgroup takes a block of
-//     R = 128 NQ consecutive rows of one sequence and one KV head, a wavefront 32 NQ of them.  K and V are shared by the whole
+//     R = 32 NW consecutive rows of one sequence and one KV head, a wavefront 32 of them.  K and V are shared by the whole
 //     group, and short chunks (drafted tokens) fill the tiles with heads.  Blocks are numbered by a prefix sum over the
 //     batch that every workgroup forms itself (the offsets are device data), the last block of a sequence first: it has the most keys.
 //   - Keys pass through LDS in tiles of KT, as f16 (or f32), once for all rows of the workgroup: global loads of tile t + 1 run
@@ -94,15 +94,15 @@ __device__ __forceinline__ void block_prefix(const PagedAttnLaunch& a, uint32_t 
     __syncthreads();
 }
 
-template <int DT, int D, bool IOF16, bool CAP, int NQ, int KT, int NW, int MINW>
+template <int DT, int D, bool IOF16, bool CAP, int KT, int CK, int NW, int MINW>
 __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnLaunch a, uint32_t n_split) {
     using Z = PreShape<DT, D, KT, NW>;
     constexpr bool F32C = DT == kF32;
     constexpr bool PAIR = !IOF16 && !F32C;                   // queries and weights as value + remainder
-    constexpr int NB = KT / 32;                              // 32-key blocks per tile
+    constexpr int NB = CK / 32;                              // 32-key blocks per chunk: what a wavefront takes through both products at once
     constexpr int DT32 = D / 32;
-    constexpr uint32_t R = 32u * NQ * NW;
-    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];   // two buffers, then the prefix sums
+    constexpr uint32_t R = 32u * NW;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];   // two buffers; before the first tile, the prefix sums
     __shared__ uint32_t wave_sum[NW];
     // keys whose V row holds an infinity or NaN, from tiles that are hidden in part: at most the tiles the block's queries and
     // the two ends of its window cut through
@@ -113,7 +113,8 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
     const int n32 = lane & 31, hf = lane >> 5;
     const uint32_t group = a.n_heads / a.c.n_kv_heads, kvh = blockIdx.x;
     const uint32_t dr = a.c.head_dim;
-    uint32_t* const pre = reinterpret_cast<uint32_t*>(lds + 2 * Z::BUF);
+    uint32_t* const pre = reinterpret_cast<uint32_t*>(lds);
+    static_assert(2 * Z::BUF >= ((int)kPagedMaxSeqs + 1) * 4, "the prefix sums fit the tile buffers");
     if (tid == 0) n_odd = 0u;
     block_prefix<NW>(a, group, R, pre, wave_sum, tid);
     const uint32_t blocks = __builtin_amdgcn_readfirstlane(pre[a.s.n_seqs]);
@@ -134,6 +135,7 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
     t1 = __builtin_amdgcn_readfirstlane(t1);
     const uint32_t n_rows = (t1 - t0) * group;               // (< 2^31 * 2^16 would not fit: the launcher refuses n_tokens * n_heads >= 2^32)
     const uint32_t row0 = (bi - __builtin_amdgcn_readfirstlane(pre[s])) * R;
+    __syncthreads();                                         // the prefix sums have been read: the buffers are free
     const uint32_t row1 = n_rows - row0 < R ? n_rows : row0 + R;
     const int kv_len = (int)__builtin_amdgcn_readfirstlane(paged_kv_len(a.s, s));
     const int pos0 = kv_len - (int)(t1 - t0);                // position of the chunk's first token
@@ -150,39 +152,37 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
     auto tile_key = [&](uint32_t t) { return (t < sink_tiles ? t : first + t - sink_tiles) * (uint32_t)KT; };
 
     // ---- this wavefront's rows
-    const uint32_t wr0 = row0 + (uint32_t)w * 32u * NQ;
+    const uint32_t wr0 = row0 + (uint32_t)w * 32u;
     const bool wave_has = wr0 < row1;
-    const uint32_t wr1 = row1 < wr0 + 32u * NQ ? row1 : wr0 + 32u * NQ;
+    const uint32_t wr1 = row1 < wr0 + 32u ? row1 : wr0 + 32u;
     const int wmin = wave_has ? pos0 + (int)(wr0 / group) : 0, wmax = wave_has ? pos0 + (int)((wr1 - 1u) / group) : -1;
     const int wlo_max = wmax > 0 ? (int)paged_window_lo(a.window, (uint32_t)wmax) : 0;     // window start of the last query
     const int wlo_min = wmin > 0 ? (int)paged_window_lo(a.window, (uint32_t)wmin) : 0;
-    uint32_t lo[NQ], span[NQ], lead[NQ];                     // a row sees the keys [lo, lo + span) and [0, lead)
-    uint32_t tok[NQ], head[NQ];
-    bool real[NQ];
-#pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-        const uint32_t r = wr0 + 32u * q + (uint32_t)n32;
-        real[q] = r < row1;
-        const uint32_t rr = real[q] ? r : row0;
-        tok[q] = rr / group;
-        head[q] = kvh * group + rr - tok[q] * group;
-        const int pos = real[q] ? pos0 + (int)tok[q] : -1;
-        lo[q] = pos > 0 ? paged_window_lo(a.window, (uint32_t)pos) : 0u;
-        span[q] = pos < 0 ? 0u : (uint32_t)pos + 1u - lo[q];
-        lead[q] = pos < 0 ? 0u : a.n_sink < (uint32_t)pos + 1u ? a.n_sink : (uint32_t)pos + 1u;
-        tok[q] += t0;
+    uint32_t lo, span, lead;                     // a row sees the keys [lo, lo + span) and [0, lead)
+    uint32_t tok, head;
+    bool real;
+    {
+        const uint32_t r = wr0 + (uint32_t)n32;
+        real = r < row1;
+        const uint32_t rr = real ? r : row0;
+        tok = rr / group;
+        head = kvh * group + rr - tok * group;
+        const int pos = real ? pos0 + (int)tok : -1;
+        lo = pos > 0 ? paged_window_lo(a.window, (uint32_t)pos) : 0u;
+        span = pos < 0 ? 0u : (uint32_t)pos + 1u - lo;
+        lead = pos < 0 ? 0u : a.n_sink < (uint32_t)pos + 1u ? a.n_sink : (uint32_t)pos + 1u;
+        tok += t0;
     }
     // ---- Q^T operands
-    half8_t qh[F32C ? 1 : NQ][F32C ? 1 : D / 16], ql[PAIR ? NQ : 1][PAIR ? D / 16 : 1];
-    float qf[F32C ? NQ : 1][F32C ? D / 2 : 1];
-#pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-        const uint64_t at = (uint64_t)tok[q] * a.q_stride + (uint64_t)head[q] * dr;
+    half8_t qh[F32C ? 1 : D / 16], ql[PAIR ? D / 16 : 1];
+    float qf[F32C ? D / 2 : 1];
+    {
+        const uint64_t at = (uint64_t)tok * a.q_stride + (uint64_t)head * dr;
         if constexpr (F32C) {
 #pragma unroll
             for (int c = 0; c < D / 8; ++c) {
                 const uint32_t d = 8u * c + 4u * (uint32_t)hf;
-                const bool ok = real[q] && d < dr;
+                const bool ok = real && d < dr;
                 float4_t x;
                 if constexpr (IOF16) {
                     const half4_t h = *reinterpret_cast<const half4_t*>(reinterpret_cast<const _Float16*>(a.q) + at + (ok ? d : 0u));
@@ -192,17 +192,17 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
                     x = *reinterpret_cast<const float4_t*>(reinterpret_cast<const float*>(a.q) + at + (ok ? d : 0u));
                 }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) qf[q][4 * c + j] = ok ? x[j] : 0.f;
+                for (int j = 0; j < 4; ++j) qf[4 * c + j] = ok ? x[j] : 0.f;
             }
         } else {
 #pragma unroll
             for (int c = 0; c < D / 16; ++c) {
                 const uint32_t d = 16u * c + 8u * (uint32_t)hf;
-                const bool ok = real[q] && d < dr;
+                const bool ok = real && d < dr;
                 if constexpr (IOF16) {
                     const half8_t x = *reinterpret_cast<const half8_t*>(reinterpret_cast<const _Float16*>(a.q) + at + (ok ? d : 0u));
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) qh[q][c][j] = ok ? x[j] : (_Float16)0.f;
+                    for (int j = 0; j < 8; ++j) qh[c][j] = ok ? x[j] : (_Float16)0.f;
                 } else {
                     const float* const src = reinterpret_cast<const float*>(a.q) + at + (ok ? d : 0u);
                     const float4_t x0 = *reinterpret_cast<const float4_t*>(src), x1 = *reinterpret_cast<const float4_t*>(src + 4);
@@ -210,25 +210,20 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
                     for (int j = 0; j < 8; ++j) {
                         const float x = ok ? (j < 4 ? x0[j & 3] : x1[j & 3]) : 0.f;
                         const _Float16 hi = (_Float16)x;
-                        qh[q][c][j] = hi;
-                        ql[q][c][j] = (_Float16)(x - (float)hi);
+                        qh[c][j] = hi;
+                        ql[c][j] = (_Float16)(x - (float)hi);
                     }
                 }
             }
         }
     }
 
-    float16_t acc[DT32][NQ];
-    float m[NQ], l[NQ];
+    float16_t acc[DT32];
+    float m = kMasked, l = 0.f;                              // l: this lane's keys only, summed at the end
 #pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-        m[q] = kMasked;
-        l[q] = 0.f;
+    for (int n = 0; n < DT32; ++n)
 #pragma unroll
-        for (int n = 0; n < DT32; ++n)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[n][q][e] = 0.f;
-    }
+        for (int e = 0; e < 16; ++e) acc[n][e] = 0.f;
     const float scale_l2 = a.scale * 1.44269504088896f;
     const float cap_l2 = a.softcap * 1.44269504088896f;
     const float inv_cap_l2 = CAP ? 1.0f / cap_l2 : 0.f;
@@ -329,36 +324,28 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
     };
 
     // ---- one tile
-    auto compute = [&](bool masked, int buf, const Pages& P, uint32_t t) {   // masked: some of the queries do not see some of the keys
-        const uint8_t* const kl = lds + buf * Z::BUF;
-        const uint8_t* const vl = kl + KT * Z::KPITCH;
-        const int kb = (int)tile_key(t);
-        float16_t sc[NB][NQ];
+    auto compute = [&](bool masked, int buf, const uint32_t (&pages)[CK / 16], int chunk_at, int kb) {   // masked: some of the queries do not see some of the keys
+        const uint8_t* const kl = lds + buf * Z::BUF + chunk_at * Z::KPITCH;
+        const uint8_t* const vl = lds + buf * Z::BUF + KT * Z::KPITCH + chunk_at * Z::VPITCH;
+        float16_t sc[NB];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
 #pragma unroll
-            for (int q = 0; q < NQ; ++q)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) sc[b][q][e] = 0.f;
+            for (int e = 0; e < 16; ++e) sc[b][e] = 0.f;
             const uint8_t* const krow = kl + (32 * b + n32) * Z::KPITCH + hf * 16;
             if constexpr (F32C) {
 #pragma unroll
                 for (int c = 0; c < D / 8; ++c) {
                     const float4_t k = *reinterpret_cast<const float4_t*>(krow + 32 * c);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-#pragma unroll
-                        for (int q = 0; q < NQ; ++q) sc[b][q] = __builtin_amdgcn_mfma_f32_32x32x2f32(k[j], qf[q][4 * c + j], sc[b][q], 0, 0, 0);
+                    for (int j = 0; j < 4; ++j) sc[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(k[j], qf[4 * c + j], sc[b], 0, 0, 0);
                 }
             } else {
 #pragma unroll
                 for (int c = 0; c < D / 16; ++c) {
                     const half8_t k = *reinterpret_cast<const half8_t*>(krow + 32 * c);
-#pragma unroll
-                    for (int q = 0; q < NQ; ++q) {
-                        sc[b][q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[q][c], sc[b][q], 0, 0, 0);
-                        if constexpr (PAIR) sc[b][q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[q][c], sc[b][q], 0, 0, 0);
-                    }
+                    sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[c], sc[b], 0, 0, 0);
+                    if constexpr (PAIR) sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[c], sc[b], 0, 0, 0);
                 }
             }
         }
@@ -366,9 +353,7 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
 #pragma unroll
             for (int b = 0; b < NB; ++b)
 #pragma unroll
-                for (int q = 0; q < NQ; ++q)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) sc[b][q][e] = softcap_l2(sc[b][q][e] * scale_l2, cap_l2, inv_cap_l2);
+                for (int e = 0; e < 16; ++e) sc[b][e] = softcap_l2(sc[b][e] * scale_l2, cap_l2, inv_cap_l2);
         }
         if (masked) {
             // key in [lo, pos] as one unsigned comparison against their number; a key among the first tokens as another
@@ -377,56 +362,42 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const bool there = P.tile[2 * b + h] < a.c.n_pages;      // (uniform: 16 keys lie in one page)
+                        const bool there = pages[2 * b + h] < a.c.n_pages;      // (uniform: 16 keys lie in one page)
+                        const uint32_t key = (uint32_t)(kb + 32 * b + 16 * h + 4 * hf), rel = key - lo;
+                        const uint32_t some = there ? span : 0u, front = there ? lead : 0u;
 #pragma unroll
-                        for (int q = 0; q < NQ; ++q) {
-                            const uint32_t key = (uint32_t)(kb + 32 * b + 16 * h + 4 * hf), rel = key - lo[q];
-                            const uint32_t some = there ? span[q] : 0u, front = there ? lead[q] : 0u;
-#pragma unroll
-                            for (uint32_t x = 0; x < 8; ++x) {
-                                const uint32_t off = 8u * (x / 4u) + x % 4u;
-                                bool seen = rel + off < some;
-                                if constexpr (decltype(firsts)::value) seen = seen || key + off < front;
-                                sc[b][q][8 * h + x] = seen ? sc[b][q][8 * h + x] : -__builtin_inff();
-                            }
+                        for (uint32_t x = 0; x < 8; ++x) {
+                            const uint32_t off = 8u * (x / 4u) + x % 4u;
+                            bool seen = rel + off < some;
+                            if constexpr (decltype(firsts)::value) seen = seen || key + off < front;
+                            sc[b][8 * h + x] = seen ? sc[b][8 * h + x] : -__builtin_inff();
                         }
                     }
             };
             if ((uint32_t)kb < a.n_sink) hide(std::true_type{}); else hide(std::false_type{});
         }
-        float mx[NQ];
-        bool raise = false;
+        float mx = sc[0][0];
 #pragma unroll
-        for (int q = 0; q < NQ; ++q) {
-            mx[q] = sc[0][q][0];
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
+            for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[b][e]);
+        if (__any(mx * fac > m + (kRaise + kBias))) {
+            const float mn = fmaxf(m, max_over_halves(mx) * fac - kBias);
+            const float corr = __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= corr;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) mx[q] = fmaxf(mx[q], sc[b][q][e]);
-            raise = raise || mx[q] * fac > m[q] + (kRaise + kBias);
-        }
-        if (__any(raise)) {
+            for (int n = 0; n < DT32; ++n)
 #pragma unroll
-            for (int q = 0; q < NQ; ++q) {
-                const float mn = fmaxf(m[q], max_over_halves(mx[q]) * fac - kBias);
-                const float corr = __builtin_amdgcn_exp2f(m[q] - mn);
-                m[q] = mn;
-                l[q] *= corr;
-#pragma unroll
-                for (int n = 0; n < DT32; ++n)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) acc[n][q][e] *= corr;
-            }
+                for (int e = 0; e < 16; ++e) acc[n][e] *= corr;
         }
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int q = 0; q < NQ; ++q)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    sc[b][q][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][q][e], fac, -m[q]));
-                    if constexpr (F32C || PAIR) l[q] += sc[b][q][e];
-                }
+            for (int e = 0; e < 16; ++e) {
+                sc[b][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][e], fac, -m));
+                if constexpr (F32C || PAIR) l += sc[b][e];
+            }
         if constexpr (F32C) {
 #pragma unroll
             for (int b = 0; b < NB; ++b)
@@ -436,41 +407,32 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
 #pragma unroll
                     for (int n = 0; n < DT32; ++n) {
                         const float v = *reinterpret_cast<const float*>(vrow + 128 * n);
-#pragma unroll
-                        for (int q = 0; q < NQ; ++q) acc[n][q] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, sc[b][q][e], acc[n][q], 0, 0, 0);
+                        acc[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, sc[b][e], acc[n], 0, 0, 0);
                     }
                 }
         } else {
             // lane's place in the transposing read: row 4 hf + (lane % 16) / 4 of eight-row steps, column group of its sixteen lanes
             const uint8_t* const vlane = vl + (4 * hf + (lane & 15) / 4) * Z::VPITCH + (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
 #pragma unroll
-            for (int kk = 0; kk < KT / 16; ++kk) {
-                half8_t ph[NQ], pl[PAIR ? NQ : 1];
+            for (int kk = 0; kk < CK / 16; ++kk) {
+                uint32_t h[4], r[4];
 #pragma unroll
-                for (int q = 0; q < NQ; ++q) {
-                    uint32_t h[4], r[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float p0 = sc[kk / 2][q][8 * (kk % 2) + 2 * i], p1 = sc[kk / 2][q][8 * (kk % 2) + 2 * i + 1];
-                        const half2_t hh = half2_t{(_Float16)p0, (_Float16)p1};
-                        h[i] = __builtin_bit_cast(uint32_t, hh);
-                        // the sum of the weights as the product uses them: their rounding cancels in the mean
-                        if constexpr (!PAIR) l[q] = __builtin_amdgcn_fdot2(hh, half2_t{(_Float16)1.f, (_Float16)1.f}, l[q], false);
-                        if constexpr (PAIR) r[i] = pack_f16_remainder(p0, p1, h[i]);
-                    }
-                    ph[q] = __builtin_bit_cast(half8_t, h);
-                    if constexpr (PAIR) pl[q] = __builtin_bit_cast(half8_t, r);
+                for (int i = 0; i < 4; ++i) {
+                    const float p0 = sc[kk / 2][8 * (kk % 2) + 2 * i], p1 = sc[kk / 2][8 * (kk % 2) + 2 * i + 1];
+                    const half2_t hh = half2_t{(_Float16)p0, (_Float16)p1};
+                    h[i] = __builtin_bit_cast(uint32_t, hh);
+                    // f16 weights: the sum is that of the weights as the product uses them, so their rounding cancels in the mean
+                    if constexpr (!PAIR) l = __builtin_amdgcn_fdot2(hh, half2_t{(_Float16)1.f, (_Float16)1.f}, l, false);
+                    if constexpr (PAIR) r[i] = pack_f16_remainder(p0, p1, h[i]);
                 }
+                const half8_t ph = __builtin_bit_cast(half8_t, h);
 #pragma unroll
                 for (int n = 0; n < DT32; ++n) {
                     const half4_t v0 = lds_read_tr16(reinterpret_cast<const _Float16*>(vlane + 16 * kk * Z::VPITCH + 64 * n));
                     const half4_t v1 = lds_read_tr16(reinterpret_cast<const _Float16*>(vlane + (16 * kk + 8) * Z::VPITCH + 64 * n));
                     const half8_t v = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-                    for (int q = 0; q < NQ; ++q) {
-                        acc[n][q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[q], acc[n][q], 0, 0, 0);
-                        if constexpr (PAIR) acc[n][q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[q], acc[n][q], 0, 0, 0);
-                    }
+                    acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph, acc[n], 0, 0, 0);
+                    if constexpr (PAIR) acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(half8_t, r), acc[n], 0, 0, 0);
                 }
             }
         }
@@ -489,13 +451,25 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
             const Pages p2 = get_pages(t + 2u);
             if (t + 1u < tb) fetch(p1, t + 1u);
             if (wave_has) {
-                const int kb = (int)tile_key(t);
-                bool ghost = false;
+                auto one = [&](int c) {
+                    const int kb = (int)tile_key(t) + c;
+                    uint32_t pages[CK / 16];
+                    bool ghost = false;
 #pragma unroll
-                for (int i = 0; i < SUBS; ++i) ghost = ghost || p0.tile[i] >= a.c.n_pages;
-                // (a tile that none of the wavefront's queries sees is passed over)
-                if (!(kb > wmax || ((uint32_t)kb >= a.n_sink && kb + KT <= wlo_min)))
-                    compute(!(kb + KT - 1 <= wmin && (kb >= wlo_max || (uint32_t)(kb + KT) <= a.n_sink) && !ghost), buf, p0, t);
+                    for (int i = 0; i < CK / 16; ++i) {
+                        pages[i] = p0.tile[i];
+#pragma unroll
+                        for (int x = 1; x < KT / CK; ++x) pages[i] = c == x * CK ? p0.tile[x * (CK / 16) + i] : pages[i];
+                        ghost = ghost || pages[i] >= a.c.n_pages;
+                    }
+                    // (a chunk that none of the wavefront's queries sees is passed over)
+                    if (!(kb > wmax || ((uint32_t)kb >= a.n_sink && kb + CK <= wlo_min)))
+                        compute(!(kb + CK - 1 <= wmin && (kb >= wlo_max || (uint32_t)(kb + CK) <= a.n_sink) && !ghost), buf, pages, c, kb);
+                };
+                if constexpr (KT == CK) one(0);
+                else
+#pragma unroll 1
+                    for (int c = 0; c < KT; c += CK) one(c);
             }
             if (t + 1u < tb) stage(buf ^ 1, p1, t + 1u);
             p0 = p1;
@@ -504,14 +478,12 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
     }
 
     // ---- output
-#pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-        const float L = xor32_sum(l[q]);
-        if (!real[q]) continue;
+    const float L = xor32_sum(l);
+    const uint64_t row = ((uint64_t)tok * a.n_heads + head) * n_split + blockIdx.z;
+    const uint64_t at = (uint64_t)tok * a.o_stride + (uint64_t)head * dr;
+    if (real) {
         const float inv = n_split > 1u ? 1.0f : L != 0.f ? 1.0f / L : 0.f;
-        const uint64_t row = ((uint64_t)tok[q] * a.n_heads + head[q]) * n_split + blockIdx.z;
-        const uint64_t at = (uint64_t)tok[q] * a.o_stride + (uint64_t)head[q] * dr;
-        if (n_split > 1u && hf == 0) { a.scratch_max[row] = m[q]; a.scratch_sum[row] = L; }
+        if (n_split > 1u && hf == 0) { a.scratch_max[row] = m; a.scratch_sum[row] = L; }
 #pragma unroll
         for (int n = 0; n < DT32; ++n)
 #pragma unroll
@@ -520,7 +492,7 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
                 if (d >= dr) continue;
                 float4_t v;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = acc[n][q][4 * b + j] * inv;
+                for (int j = 0; j < 4; ++j) v[j] = acc[n][4 * b + j] * inv;
                 if (n_split > 1u) {
                     *reinterpret_cast<float4_t*>(a.scratch_out + row * dr + d) = v;
                 } else if constexpr (IOF16) {
@@ -542,31 +514,26 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
         const uint32_t key = __builtin_amdgcn_readfirstlane(odd_key[i]);
         const uint32_t page = (uint32_t)table[key >> a.c.page_shift];
         const uint8_t* const vrow = a.c.v + (uint64_t)(page < a.c.n_pages ? page : 0u) * a.c.page_bytes + (head_rows + (key & slot_mask)) * row_b;
-#pragma unroll
-        for (int q = 0; q < NQ; ++q) {
-            if (!real[q] || !(key - lo[q] < span[q] || key < lead[q])) continue;
-            const uint64_t row = ((uint64_t)tok[q] * a.n_heads + head[q]) * n_split + blockIdx.z;
-            const uint64_t at = (uint64_t)tok[q] * a.o_stride + (uint64_t)head[q] * dr;
+        if (!real || !(key - lo < span || key < lead)) continue;
 #pragma unroll 1
-            for (uint32_t d = 4u * (uint32_t)hf; d < dr; d += 8u)
+        for (uint32_t d = 4u * (uint32_t)hf; d < dr; d += 8u)
 #pragma unroll 1
-                for (uint32_t j = d; j < d + 4u; ++j) {
-                    const float v = load_kv_elem(vrow, DT, j);
-                    if (fabsf(v) < __builtin_inff()) continue;
-                    if (n_split > 1u) a.scratch_out[row * dr + j] += v;
-                    else if constexpr (IOF16) reinterpret_cast<_Float16*>(a.o)[at + j] = (_Float16)((float)reinterpret_cast<_Float16*>(a.o)[at + j] + v);
-                    else reinterpret_cast<float*>(a.o)[at + j] += v;
-                }
-        }
+            for (uint32_t j = d; j < d + 4u; ++j) {
+                const float v = load_kv_elem(vrow, DT, j);
+                if (fabsf(v) < __builtin_inff()) continue;
+                if (n_split > 1u) a.scratch_out[row * dr + j] += v;
+                else if constexpr (IOF16) reinterpret_cast<_Float16*>(a.o)[at + j] = (_Float16)((float)reinterpret_cast<_Float16*>(a.o)[at + j] + v);
+                else reinterpret_cast<float*>(a.o)[at + j] += v;
+            }
     }
 }
 
 namespace {
 
-template <int DT, int D, bool IOF16, bool CAP, int NQ, int KT, int NW, int MINW>
+template <int DT, int D, bool IOF16, bool CAP, int KT, int CK, int NW, int MINW>
 hipError_t launch_pre(const PagedAttnLaunch& L, hipStream_t stream) {
     using Z = PreShape<DT, D, KT, NW>;
-    constexpr uint64_t R = 32u * NQ * NW;
+    constexpr uint64_t R = 32u * NW;
     const uint64_t group = L.n_heads / L.c.n_kv_heads;
     // a sequence's last block may be ragged: at most one block more per sequence that has rows
     const uint64_t with_rows = L.s.n_seqs < L.s.n_tokens ? L.s.n_seqs : L.s.n_tokens;
@@ -584,8 +551,8 @@ hipError_t launch_pre(const PagedAttnLaunch& L, hipStream_t stream) {
     if (n > fits) n = fits;
     if (n > 64u) n = 64u;
     if (n == 0u) n = 1u;
-    hipLaunchKernelGGL((paged_prefill_kernel<DT, D, IOF16, CAP, NQ, KT, NW, MINW>), dim3(L.c.n_kv_heads, (uint32_t)blocks, (uint32_t)n), dim3(NW * 64),
-                       2u * Z::BUF + (L.s.n_seqs + 1u) * 4u, stream, L, (uint32_t)n);
+    hipLaunchKernelGGL((paged_prefill_kernel<DT, D, IOF16, CAP, KT, CK, NW, MINW>), dim3(L.c.n_kv_heads, (uint32_t)blocks, (uint32_t)n), dim3(NW * 64),
+                       2u * Z::BUF, stream, L, (uint32_t)n);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || n == 1u) return e;
     return launch_paged_rows_merge(L, (uint32_t)n, stream);
@@ -595,15 +562,15 @@ template <int DT, bool IOF16, bool CAP>
 hipError_t launch_dim(const PagedAttnLaunch& L, hipStream_t stream) {
     const uint32_t d = L.c.head_dim;
     if constexpr (DT == kF32) {
-        if (d <= 64u) return launch_pre<DT, 64, IOF16, CAP, 1, 32, 4, 2>(L, stream);
-        if (d <= 128u) return launch_pre<DT, 128, IOF16, CAP, 1, 32, 4, 2>(L, stream);
-        return launch_pre<DT, 256, IOF16, CAP, 1, 32, 4, 1>(L, stream);
+        if (d <= 64u) return launch_pre<DT, 64, IOF16, CAP, 32, 32, 4, 2>(L, stream);
+        if (d <= 128u) return launch_pre<DT, 128, IOF16, CAP, 32, 32, 4, 2>(L, stream);
+        return launch_pre<DT, 256, IOF16, CAP, 32, 32, 4, 1>(L, stream);
     } else {
         const bool many = (uint64_t)L.s.n_tokens * (L.n_heads / L.c.n_kv_heads) >= 256ull * L.s.n_seqs;
-        constexpr int KT = IOF16 ? 64 : 32;
-        if (d <= 64u) return many ? launch_pre<DT, 64, IOF16, CAP, 1, 64, 8, 2>(L, stream) : launch_pre<DT, 64, IOF16, CAP, 1, 64, 4, 2>(L, stream);
-        if (d <= 128u) return many ? launch_pre<DT, 128, IOF16, CAP, 1, KT, 8, 2>(L, stream) : launch_pre<DT, 128, IOF16, CAP, 1, KT, 4, 2>(L, stream);
-        return launch_pre<DT, 256, IOF16, CAP, 1, 32, 4, 1>(L, stream);
+        constexpr int CK = IOF16 ? 64 : 32, KT = 64;
+        if (d <= 64u) return many ? launch_pre<DT, 64, IOF16, CAP, 64, 64, 8, 2>(L, stream) : launch_pre<DT, 64, IOF16, CAP, 64, 64, 4, 2>(L, stream);
+        if (d <= 128u) return many ? launch_pre<DT, 128, IOF16, CAP, KT, CK, 8, 2>(L, stream) : launch_pre<DT, 128, IOF16, CAP, KT, CK, 4, 2>(L, stream);
+        return launch_pre<DT, 256, IOF16, CAP, 32, 32, 4, 1>(L, stream);
     }
 }
 
