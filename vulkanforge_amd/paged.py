@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+from array import array
 from dataclasses import dataclass
 from typing import List, Optional, Sequence
 
@@ -30,17 +31,39 @@ class PagedKvConfig:
 
 def _pages(values: Sequence[int]):
     """Page list -> uint32 array (-1 becomes VFKV_NO_PAGE)."""
-    return (C.c_uint32 * max(len(values), 1))(*[v & 0xFFFFFFFF for v in values])
+    try:
+        a = array("I", values)
+    except OverflowError:
+        a = array("I", [v & 0xFFFFFFFF for v in values])
+    return (C.c_uint32 * len(a)).from_buffer(a) if a else (C.c_uint32 * 1)()
 
 
-def _list(arr, n: int) -> List[int]:
-    return [NO_PAGE if v == _ffi.NO_PAGE else v for v in arr[:n]]
+def _list(arr, lo: int, hi: int) -> List[int]:
+    out = arr[lo:hi]
+    return [NO_PAGE if v == _ffi.NO_PAGE else v for v in out] if _ffi.NO_PAGE in out else out
 
 
-def _stream(stream) -> int:
+_IO: dict = {}           # torch dtype -> io_dtype, filled on first use (the package imports without torch)
+_raw_stream = None
+
+
+def _first_use() -> None:
+    global _raw_stream
+    import torch
+    _IO.update({torch.float32: 0, torch.float16: 1})
+    # the stream's handle without building a Stream object: a decode step calls this once per layer and operator
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    _raw_stream = raw or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
+def _stream(stream, device=None) -> int:
     if stream is None:
-        import torch
-        return torch.cuda.current_stream().cuda_stream
+        if _raw_stream is None:
+            _first_use()
+        if device is None:
+            import torch
+            device = torch.cuda.current_device()
+        return _raw_stream(device)
     return stream if isinstance(stream, int) else stream.cuda_stream
 
 
@@ -135,13 +158,13 @@ class PagedKvCache:
         out = (C.c_uint32 * max(used * n_forks, 1))()
         _ffi.check(_ffi.lib().vfkv_pages_fork(self._h, _pages(pages[:used]), kv_len, n_forks, out,
                                               _stream(stream) if self.k_ptr else None))
-        return [_list(out[i * used:(i + 1) * used], used) for i in range(n_forks)]
+        return [_list(out, i * used, (i + 1) * used) for i in range(n_forks)]
 
     def compact(self, stream=None) -> List[int]:
         """Moves the live pages into the lowest ids; returns every page's new id (-1: the page was free)."""
         out = (C.c_uint32 * self.config.n_pages)()
         _ffi.check(_ffi.lib().vfkv_pages_compact(self._h, out, _stream(stream) if self.k_ptr else None))
-        return _list(out, self.config.n_pages)
+        return _list(out, 0, self.config.n_pages)
 
 
 def _int32(t, name: str):
@@ -172,7 +195,7 @@ class SeqBatch:
         self.page_table, self.kv_lens = _int32(page_table, "page_table"), _int32(kv_lens, "kv_lens")
         self.q_offsets = None if q_offsets is None else _int32(q_offsets, "q_offsets")
         self.n_seqs, self.n_tokens = n, n_tokens
-        self.device = kv_lens.device
+        self.device, self.index = kv_lens.device, kv_lens.get_device()
         self._args = _ffi.SeqBatchArgs(self.page_table.data_ptr(), self.kv_lens.data_ptr(),
                                        None if q_offsets is None else self.q_offsets.data_ptr(), n, page_table.shape[1],
                                        n_tokens, max_kv_len)
@@ -216,38 +239,33 @@ class PagedForward:
     one projection's output)."""
 
     def __init__(self, cache: PagedKvCache, n_heads: int, workspace: Optional[PagedWorkspace] = None):
-        self.cache, self.n_heads = cache, n_heads
+        self.cache, self.n_heads, self.head_dim = cache, n_heads, cache.config.head_dim
         self.workspace = workspace or PagedWorkspace(cache, n_heads)
         self.attn_scale = 1.0 / math.sqrt(cache.config.head_dim)
 
     def _rows(self, t, heads: int, batch: SeqBatch, name: str):
         """(address, elements between two tokens, io dtype) of a row tensor."""
-        if t.dim() != 3 or t.shape[0] != batch.n_tokens or t.shape[1] != heads or t.shape[2] != self.cache.config.head_dim:
-            raise ValueError(f"{name}: expected [{batch.n_tokens}, {heads}, {self.cache.config.head_dim}], got {list(t.shape)}")
-        if t.device != batch.device:
-            raise ValueError(f"{name} is on {t.device}, the batch on {batch.device}")
-        d = t.element_size()
-        if d == 4:
-            io = 0
-        elif d == 2:
-            io = 1
-        else:
-            io = -1
-        if io < 0 or str(t.dtype) != ("torch.float32", "torch.float16")[io]:
-            raise ValueError(f"{name}: float32 or float16, got {t.dtype}")
+        dim = self.head_dim
+        io = _IO.get(t.dtype)
+        if io is None or t.get_device() != batch.index or t.shape != (batch.n_tokens, heads, dim):
+            if not _IO:
+                _first_use()
+                return self._rows(t, heads, batch, name)
+            raise ValueError(f"{name}: expected [{batch.n_tokens}, {heads}, {dim}], float32 or float16, on {batch.device}; got "
+                             f"{list(t.shape)}, {t.dtype}, on {t.device}")
         token, head, elem = t.stride()
-        if (elem != 1 and t.shape[2] > 1) or (head != t.shape[2] and heads > 1):
+        if (elem != 1 and dim > 1) or (head != dim and heads > 1):
             raise ValueError(f"{name}: the heads of a token must be contiguous")
-        if t.shape[0] <= 1:
-            token = heads * t.shape[2]
-        if not heads * t.shape[2] <= token <= 0xFFFFFFFF:
+        if batch.n_tokens <= 1:
+            token = heads * dim
+        if not heads * dim <= token <= 0xFFFFFFFF:
             raise ValueError(f"{name}: tokens overlap or are too far apart (stride {token})")
         return t.data_ptr(), token, io
 
     def _dev(self, t, shape, dtype: str, batch: SeqBatch, name: str) -> Optional[int]:
         if t is None:
             return None
-        if tuple(t.shape) != shape or str(t.dtype) != dtype or not t.is_contiguous() or t.device != batch.device:
+        if t.shape != shape or not t.is_contiguous() or t.get_device() != batch.index or str(t.dtype) != dtype:
             raise ValueError(f"{name}: expected a contiguous {dtype} tensor of shape {shape} on {batch.device}")
         return t.data_ptr()
 
@@ -273,7 +291,7 @@ class PagedForward:
                            self._dev(freq_factors, (half,), "torch.float32", batch, "freq_factors"),
                            self.n_heads, io, qs or 0, os_ or 0, ks, vs)
         _ffi.check(_ffi.lib().vfkv_paged_qk_rope_kv_write(self.cache.handle, layer, batch.args, C.byref(r), rope.args,
-                                                          _stream(stream)))
+                                                          _stream(stream, batch.index)))
 
     def _attention(self, fn, layer, batch, q, o, window, n_sink, scale, softcap, stream) -> None:
         qp, qs, io = self._rows(q, self.n_heads, batch, "q")
@@ -283,7 +301,7 @@ class PagedForward:
         if window < 0 or n_sink < 0:
             raise ValueError("window and n_sink must not be negative")
         p = _ffi.PagedAttnParams(self.n_heads, window, n_sink, io, qs, os_, self.attn_scale if scale is None else scale, softcap)
-        _ffi.check(fn(self.cache.handle, layer, batch.args, C.byref(p), qp, op, self.workspace.handle, _stream(stream)))
+        _ffi.check(fn(self.cache.handle, layer, batch.args, C.byref(p), qp, op, self.workspace.handle, _stream(stream, batch.index)))
 
     def decode_attention(self, layer: int, batch: SeqBatch, q, o, window: int = 0, n_sink: int = 0,
                          scale: Optional[float] = None, softcap: float = 0.0, stream=None) -> None:
