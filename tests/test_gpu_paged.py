@@ -518,7 +518,7 @@ def serve(steps, capture, io=torch.float32):
         fwd.qk_rope_kv_write(l, batch, x[:, :hq], x[:, hq:hq + hkv], x[:, hq + hkv:], rope, q_out=q)
         fwd.prefill_attention(l, batch, q, o[l], window=24, n_sink=4)
     outs = [o.clone()]
-    forks = c.fork(lists[1], lens[1], 2)
+    forks = c.fork(lists[1], lens[1], 2).tolist()
     c.release(lists[1])
     lists, lens = [lists[0]] + forks, [lens[0], lens[1], lens[1]]
     tab, kv = table(lists), torch.tensor(lens, dtype=torch.int32, device=DEV)

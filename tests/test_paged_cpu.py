@@ -69,6 +69,9 @@ def test_retain_and_release_count_repetitions_and_undo_on_errors():
     with pytest.raises(vf.VfkvError):
         c.retain([0, 4])
     assert c.refcount(0) == 3
+    for bad in ([-2], [1 << 32], [0.5]):
+        with pytest.raises(ValueError):
+            c.release(bad)
     c.release([0, 0, 0, -1, 2, 2])                       # to zero in one call: one free page each
     assert c.free_count == 5 and c.alloc(5) == [0, 2, 3, 4, 5]
 
@@ -78,7 +81,7 @@ def test_fork_shares_full_pages_and_owns_the_last(kv, fresh):
     c = pool(12)
     used = c.pages_for(kv)
     mine = c.alloc(used)
-    a, b = c.fork(mine, kv, 2)
+    a, b = c.fork(mine, kv, 2).tolist()
     full = kv // 16
     assert a[:full] == b[:full] == mine[:full] and len(a) == used
     assert [c.refcount(p) for p in mine[:full]] == [3] * full
@@ -100,11 +103,11 @@ def test_fork_refusals_change_nothing():
         c.fork([0, 4, 2], 40, 1)                         # page 4 is free
     with pytest.raises(ValueError):
         c.fork(mine[:2], 40, 1)
-    assert c.fork(mine, 40, 0) == []
+    assert c.fork(mine, 40, 0).shape == (0, 3)
     assert c.free_count == 2 and [c.refcount(p) for p in mine] == [1, 1, 1]
-    t = c.fork([-1, 1, 2], 40, 1)[0]                     # the first page has left the window
+    t = c.fork([-1, 1, 2], 40, 1)[0].tolist()                     # the first page has left the window
     assert t[0] == -1 and t[1] == 1 and t[2] == 3
-    t = c.fork([0, 1, -1], 40, 1)[0]
+    t = c.fork([0, 1, -1], 40, 1)[0].tolist()
     assert t == [0, 1, -1]
 
 

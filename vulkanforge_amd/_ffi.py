@@ -150,12 +150,12 @@ SIGNATURES = {
     "vfkv_pages_offset_bytes": (_u64, [_vp, _u32, _u32]),
     "vfkv_pages_free_count": (_u32, [_vp]),
     "vfkv_pages_refcount": (_u32, [_vp, _u32]),
-    "vfkv_pages_alloc": (C.c_int, [_vp, _u32, _u32p]),
-    "vfkv_pages_retain": (C.c_int, [_vp, _u32p, _u32]),
-    "vfkv_pages_release": (C.c_int, [_vp, _u32p, _u32]),
-    "vfkv_pages_copy": (C.c_int, [_vp, _u32p, _u32p, _u32p, _u32, _vp]),
-    "vfkv_pages_fork": (C.c_int, [_vp, _u32p, _u32, _u32, _u32p, _vp]),
-    "vfkv_pages_compact": (C.c_int, [_vp, _u32p, _vp]),
+    "vfkv_pages_alloc": (C.c_int, [_vp, _u32, _vp]),
+    "vfkv_pages_retain": (C.c_int, [_vp, _vp, _u32]),
+    "vfkv_pages_release": (C.c_int, [_vp, _vp, _u32]),
+    "vfkv_pages_copy": (C.c_int, [_vp, _vp, _vp, _vp, _u32, _vp]),
+    "vfkv_pages_fork": (C.c_int, [_vp, _vp, _u32, _u32, _vp, _vp]),
+    "vfkv_pages_compact": (C.c_int, [_vp, _vp, _vp]),
     "vfkv_paged_qk_rope_kv_write": (C.c_int, [_vp, _u32, C.POINTER(SeqBatchArgs), C.POINTER(PagedRows), C.POINTER(MRopeParams), _vp]),
     "vfkv_paged_workspace_create": (C.c_int, [_vp, _u32, C.POINTER(_vp)]),
     "vfkv_paged_decode_attention": (C.c_int, [_vp, _u32, C.POINTER(SeqBatchArgs), C.POINTER(PagedAttnParams), _vp, _vp, _vp, _vp]),

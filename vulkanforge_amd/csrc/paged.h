@@ -78,6 +78,16 @@ uint32_t paged_decode_wgs(uint32_t head_groups);
 hipError_t launch_paged_generic(const PagedAttnLaunch& L, hipStream_t stream);
 
 #ifdef __HIPCC__
+// Logit soft-cap in log2 units, cap * tanh(y / cap), to a few steps of f32 at every size: the truncated continued fraction of tanh
+// (7 / 5 terms, 8e-9 relative) below 0.8, 1 - 2 / (exp(2 x) + 1) on the hardware exponential and reciprocal above.  (The second alone
+// is off by 1e-7 absolute, which a cap of 50 turns into 5e-6 of a score.)
+__device__ __forceinline__ float paged_softcap_l2(float y, float cap_l2, float inv_cap_l2) {
+    const float x = fabsf(y * inv_cap_l2), a = x * x;
+    const float near = x * __builtin_fmaf(a, a + 105.f, 945.f) * __builtin_amdgcn_rcpf(__builtin_fmaf(a, __builtin_fmaf(a, 15.f, 420.f), 945.f));
+    const float t = __builtin_amdgcn_exp2f(x * 2.88539008177793f);       // exp(2 x)
+    const float far = __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(t + 1.0f), 1.0f);
+    return copysignf(cap_l2 * (x < 0.8f ? near : far), y);
+}
 // Length of sequence s, within what its page table can hold.
 __device__ __forceinline__ uint32_t paged_kv_len(const PagedSeqs& S, uint32_t s) {
     const int32_t n = S.kv_lens[s];

@@ -3,8 +3,8 @@
 // o = sum_j softmax_j(scale q.k_j) v_j per head; bound by reading K and V once (4 flop per element and query head against 1, 2 or 4
 // bytes), so the kernel is built around keeping loads in flight on every CU whatever the lengths are:
 //
-//   - The keys of ALL sequences, cut into units of 16 * SUB aligned positions (first tokens, then the window), are one line of U
-//     units per KV head.  Workgroup w of N owns units [w U / N, (w + 1) U / N): every workgroup has the same work to one unit, a
+//   - The keys of ALL sequences, cut into units of 16 * SUB aligned positions (first tokens, then the window), with a few units in
+//     front of each sequence for what beginning it costs, are one line of U units per KV head.  Workgroup w of N owns units [w U / N, (w + 1) U / N): every workgroup has the same work to one unit, a
 //     long sequence is spread over many workgroups and short ones are packed.  A workgroup's range touches at most two
 //     sequences partly (its first and its last); those parts leave unnormalised sums that paged_merge_kernel joins, sequences
 //     inside the range are written directly.  The lengths are device data, so each workgroup finds its range itself
@@ -32,6 +32,9 @@ namespace {
 constexpr int kDecWaves = 4;
 constexpr int kDecHeads = 8;               // query heads of a KV head per workgroup
 constexpr float kRaise = 8.f, kBias = 6.f;  // log2
+// What beginning a sequence costs a workgroup (queries, page numbers, the join of its wavefronts), in units: it stands in front of
+// the sequence's own units in the line.  Without it 124 sequences of 7 to 11 keys went to 16 workgroups of eight each.
+constexpr uint32_t kBegin = 2u * kDecWaves;
 
 template <int DT, int D, int SUB_>
 struct DecShape {
@@ -63,10 +66,10 @@ __device__ __forceinline__ SeqUnits seq_units(uint32_t n, uint32_t window, uint3
     return r;
 }
 
-// Workgroups that share U units: the launch's, or as many as get two units per wavefront.  Never more than U, so that no range is
-// empty; 0 for an empty batch.
+// Workgroups that share a line of U units: the launch's, or as many as get two units per wavefront besides a sequence's beginning.
+// Never more than U, so that no range is empty; 0 for an empty batch.
 __device__ __forceinline__ uint32_t used_wgs(uint32_t U, uint32_t n_wg) {
-    const uint32_t most = (U + 2u * kDecWaves - 1u) / (2u * kDecWaves);
+    const uint32_t most = (U + kBegin + 2u * kDecWaves - 1u) / (kBegin + 2u * kDecWaves);
     return most < n_wg ? most : n_wg;
 }
 
@@ -83,14 +86,17 @@ __device__ __forceinline__ float ror8_sum(float x) { return x + dpp_f<kDppRor8>(
 
 }  // namespace
 
-// Prefix sums of the units: pre[s] for s <= n_seqs, by the whole workgroup.
+// Length of a sequence in the line of units.
+__device__ __forceinline__ uint32_t line_units(uint32_t units) { return units ? units + kBegin : 0u; }
+
+// Prefix sums of the line: pre[s] for s <= n_seqs, by the whole workgroup.
 template <int UK>
 __device__ __forceinline__ void unit_prefix(const PagedAttnLaunch& a, uint32_t* pre, uint32_t* wave_sum, int tid) {
     const int lane = tid & 63, w = tid >> 6;
     uint32_t carry = 0u;
     for (uint32_t base = 0; base < a.s.n_seqs; base += 256u) {
         const uint32_t s = base + (uint32_t)tid;
-        uint32_t x = s < a.s.n_seqs ? seq_units(paged_kv_len(a.s, s), a.window, a.n_sink, UK).units : 0u;
+        uint32_t x = s < a.s.n_seqs ? line_units(seq_units(paged_kv_len(a.s, s), a.window, a.n_sink, UK).units) : 0u;
         const uint32_t mine = x;
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) {
@@ -113,7 +119,7 @@ __device__ __forceinline__ void unit_prefix(const PagedAttnLaunch& a, uint32_t* 
 }
 
 template <int DT, int D, int SUB>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_decode_kernel(PagedAttnLaunch a, uint32_t n_wg, uint32_t slices) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_decode_kernel(PagedAttnLaunch a, uint32_t n_wg, uint32_t slices, uint32_t direct) {
     using Z = DecShape<DT, D, SUB>;
     constexpr int OP = D + 4;                                            // pitch of an output row in LDS
     __shared__ __attribute__((aligned(16))) float o_lds[kDecWaves][kDecHeads][OP];
@@ -130,22 +136,27 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_decode_kernel(Pag
     const uint32_t h0 = kvh * group + slice * kDecHeads;
     const uint32_t heads = group - slice * kDecHeads < (uint32_t)kDecHeads ? group - slice * kDecHeads : (uint32_t)kDecHeads;
     const uint32_t dr = a.c.head_dim;
-    unit_prefix<Z::UK>(a, pre, wave_sum, tid);
-    const uint32_t U = pre[a.s.n_seqs];
-    // sequences without a key: zeros
-    for (uint32_t s = wg; s < a.s.n_seqs; s += n_wg) {
-        if (pre[s + 1u] != pre[s]) continue;
+    auto no_keys = [&](uint32_t s) {                                      // a sequence without a key: zeros
         for (uint32_t e = tid; e < heads * dr; e += 256u) {
             const uint64_t at = (uint64_t)s * a.o_stride + (uint64_t)h0 * dr + e;
             if (a.io_f16) reinterpret_cast<_Float16*>(a.o)[at] = (_Float16)0.f; else reinterpret_cast<float*>(a.o)[at] = 0.f;
         }
-    }
-    const uint32_t n_eff = used_wgs(U, n_wg);
-    if (wg >= n_eff) return;
-    const uint32_t u0 = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)wg * U / n_eff));
-    const uint32_t u1 = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)(wg + 1u) * U / n_eff));
-    uint32_t s_first;
-    {
+    };
+    uint32_t u0 = 0u, u1, s_first, s_end = a.s.n_seqs;
+    if (direct) {
+        s_first = wg;
+        s_end = wg + 1u;
+        u1 = line_units(seq_units(__builtin_amdgcn_readfirstlane(paged_kv_len(a.s, wg)), a.window, a.n_sink, Z::UK).units);
+        if (u1 == 0u) { no_keys(wg); return; }
+    } else {
+        unit_prefix<Z::UK>(a, pre, wave_sum, tid);
+        const uint32_t U = pre[a.s.n_seqs];
+        for (uint32_t s = wg; s < a.s.n_seqs; s += n_wg)
+            if (pre[s + 1u] == pre[s]) no_keys(s);
+        const uint32_t n_eff = used_wgs(U, n_wg);
+        if (wg >= n_eff) return;
+        u0 = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)wg * U / n_eff));
+        u1 = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)(wg + 1u) * U / n_eff));
         uint32_t x = 0u, y = a.s.n_seqs - 1u;                            // the last s with pre[s] <= u0 (it has units)
         while (x < y) {
             const uint32_t mid = (x + y + 1u) >> 1;
@@ -180,12 +191,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_decode_kernel(Pag
         uint32_t p[SUB];
     };
 
-    for (uint32_t s = s_first; s < a.s.n_seqs; ++s) {
-        const uint32_t ps = __builtin_amdgcn_readfirstlane(pre[s]), pe = __builtin_amdgcn_readfirstlane(pre[s + 1u]);
+    for (uint32_t s = s_first; s < s_end; ++s) {
+        const uint32_t ps = direct ? 0u : __builtin_amdgcn_readfirstlane(pre[s]), pe = direct ? u1 : __builtin_amdgcn_readfirstlane(pre[s + 1u]);
         if (ps >= u1) break;
         if (ps == pe) continue;
         const SeqUnits Q = seq_units(__builtin_amdgcn_readfirstlane(paged_kv_len(a.s, s)), a.window, a.n_sink, Z::UK);
-        const uint32_t ua = (ps > u0 ? ps : u0) - ps, ub = (pe < u1 ? pe : u1) - ps;   // units [ua, ub) of the sequence
+        // this range's part of the sequence, units [ua, ub)
+        const uint32_t la = (ps > u0 ? ps : u0) - ps, lb = (pe < u1 ? pe : u1) - ps;
+        const uint32_t ua = la > kBegin ? la - kBegin : 0u, ub = lb > kBegin ? lb - kBegin : 0u;
+        if (ua >= ub) continue;
         const int32_t* const table = a.s.table + (uint64_t)s * a.s.table_stride;
 
         // ---- q' as the B operand of the first product
@@ -314,7 +328,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_decode_kernel(Pag
 #pragma unroll
                 for (int t = 0; t < SUB; ++t)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) x[t][i] = softcap_l2(x[t][i], cap_l2, inv_cap_l2);
+                    for (int i = 0; i < 4; ++i) x[t][i] = paged_softcap_l2(x[t][i], cap_l2, inv_cap_l2);
             }
             if (!full) {
 #pragma unroll
@@ -449,7 +463,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_decode_kernel(Pag
             if (g == 0) { m_lds[w][col] = m; l_lds[w][col] = l; }
         }
         __syncthreads();
-        const bool whole = ua == 0u && ub == pe - ps;
+        const bool whole = ua == 0u && ub == Q.units;
         const uint64_t part = (uint64_t)wg * 2u + (s == s_first ? 0u : 1u);
         for (uint32_t e = tid; e < heads * (D / 4); e += 256u) {
             const uint32_t h = e / (D / 4), d = (e % (D / 4)) * 4u;
@@ -499,10 +513,10 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnLaunch a, uin
     __shared__ float ls[256];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const uint32_t head = blockIdx.x, s = blockIdx.y;
-    const uint32_t mine = seq_units(paged_kv_len(a.s, s), a.window, a.n_sink, uk).units;
+    const uint32_t mine = line_units(seq_units(paged_kv_len(a.s, s), a.window, a.n_sink, uk).units);
     uint32_t before = 0u, all = 0u;
     for (uint32_t t = tid; t < a.s.n_seqs; t += 256u) {
-        const uint32_t x = seq_units(paged_kv_len(a.s, t), a.window, a.n_sink, uk).units;
+        const uint32_t x = line_units(seq_units(paged_kv_len(a.s, t), a.window, a.n_sink, uk).units);
         all += x;
         before += t < s ? x : 0u;
     }
@@ -518,7 +532,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnLaunch a, uin
     if (mine == 0u) return;
     // workgroup of unit u: the largest w with w U / N <= u
     n_wg = used_wgs(U, n_wg);
-    const uint32_t wa = (uint32_t)((((uint64_t)before + 1u) * n_wg - 1u) / U);
+    const uint32_t wa = (uint32_t)((((uint64_t)before + kBegin + 1u) * n_wg - 1u) / U);   // of its first unit
     const uint32_t wb = (uint32_t)((((uint64_t)before + mine) * n_wg - 1u) / U);
     if (wa == wb) return;                                                // written by the workgroup itself
     const uint32_t dr = a.c.head_dim, quads = dr / 4u;
@@ -578,14 +592,19 @@ hipError_t launch_dec(const PagedAttnLaunch& L, hipStream_t stream) {
     // an upper bound of the units from what the host knows
     uint64_t keys = L.max_kv;
     if (L.window != 0u && (uint64_t)L.window + L.n_sink + 2u * UK < keys) keys = (uint64_t)L.window + L.n_sink + 2u * UK;
-    const uint64_t units = (uint64_t)L.s.n_seqs * ((keys + UK - 1u) / UK);
+    const uint64_t per_seq = (keys + UK - 1u) / UK;
+    // Short sequences (up to four units per wavefront): a workgroup each, without the prefix sums and without a join.
+    if (per_seq <= 4u * kDecWaves) {
+        hipLaunchKernelGGL((paged_decode_kernel<DT, D, SUB>), dim3(n_hg, L.s.n_seqs), dim3(256), 0, stream, L, L.s.n_seqs, slices, 1u);
+        return hipGetLastError();
+    }
     uint64_t n = paged_decode_wgs(n_hg);
-    const uint64_t useful = (units + 2u * kDecWaves - 1u) / (2u * kDecWaves);   // at least two units per wavefront
+    const uint64_t useful = (L.s.n_seqs * (per_seq + kBegin) + kBegin + 2u * kDecWaves - 1u) / (kBegin + 2u * kDecWaves);
     if (n > useful) n = useful;
     const uint64_t fits = L.scratch_rows / (2u * (uint64_t)L.n_heads);
     if (n > fits) n = fits;
     if (n == 0u) n = 1u;
-    hipLaunchKernelGGL((paged_decode_kernel<DT, D, SUB>), dim3(n_hg, (uint32_t)n), dim3(256), (L.s.n_seqs + 1u) * 4u, stream, L, (uint32_t)n, slices);
+    hipLaunchKernelGGL((paged_decode_kernel<DT, D, SUB>), dim3(n_hg, (uint32_t)n), dim3(256), (L.s.n_seqs + 1u) * 4u, stream, L, (uint32_t)n, slices, 0u);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || n == 1u) return e;
     hipLaunchKernelGGL(paged_merge_kernel, dim3(L.n_heads, L.s.n_seqs), dim3(256), 0, stream, L, (uint32_t)n, UK);

@@ -353,7 +353,7 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
 #pragma unroll
             for (int b = 0; b < NB; ++b)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) sc[b][e] = softcap_l2(sc[b][e] * scale_l2, cap_l2, inv_cap_l2);
+                for (int e = 0; e < 16; ++e) sc[b][e] = paged_softcap_l2(sc[b][e] * scale_l2, cap_l2, inv_cap_l2);
         }
         if (masked) {
             // key in [lo, pos] as one unsigned comparison against their number; a key among the first tokens as another
@@ -540,13 +540,15 @@ hipError_t launch_pre(const PagedAttnLaunch& L, hipStream_t stream) {
     uint64_t blocks = L.s.n_tokens * group / R + with_rows;
     if (blocks > L.s.n_tokens * group) blocks = L.s.n_tokens * group;
     if (blocks > 65535u * 4096ull) return hipErrorInvalidValue;
-    // split over the keys: as long as the card has room, at least four tiles per part
+    // split over the keys: as long as the card has room, at least 128 keys per part (F32 pages: 32, a tile is longer work there
+    // than the join)
+    constexpr uint64_t least = DT == kF32 ? 32u : 128u;
     const uint64_t likely = (L.s.n_tokens * group + R - 1u) / R * L.c.n_kv_heads;
     const uint64_t room = 256u * MINW * 4u / NW;
     uint64_t keys = L.max_kv;
     if (L.window != 0u && (uint64_t)L.window + L.n_sink + R + 2u * KT < keys) keys = (uint64_t)L.window + L.n_sink + R + 2u * KT;
     uint64_t n = room / likely;
-    if (n > keys / (4u * KT)) n = keys / (4u * KT);
+    if (n > keys / least) n = keys / least;
     const uint64_t fits = L.scratch_rows / ((uint64_t)L.s.n_tokens * L.n_heads);
     if (n > fits) n = fits;
     if (n > 64u) n = 64u;

@@ -12,6 +12,8 @@ from array import array
 from dataclasses import dataclass
 from typing import List, Optional, Sequence
 
+import numpy as np
+
 from . import _ffi
 from .forward import Workspace
 from .kv_cache import KvDtype
@@ -29,18 +31,30 @@ class PagedKvConfig:
     dtype: KvDtype = KvDtype.F16
 
 
-def _pages(values: Sequence[int]):
-    """Page list -> uint32 array (-1 becomes VFKV_NO_PAGE)."""
+def _pages(values):
+    """Page list (a sequence of whole numbers or a numpy array) -> unsigned 32-bit array; -1 becomes VFKV_NO_PAGE."""
+    if isinstance(values, np.ndarray):
+        if values.size and values.dtype.kind not in "iu":
+            raise ValueError("pages are whole numbers")
+        if values.size > 256:                            # (below, numpy's calls cost more than the list)
+            if values.min() < -1 or values.max() > _ffi.NO_PAGE:
+                raise ValueError("a page number does not fit")
+            return np.ascontiguousarray(values.astype(np.uint32).reshape(-1))
+        values = values.reshape(-1).tolist()
     try:
-        a = array("I", values)
+        return array("I", values)
+    except TypeError:
+        raise ValueError("pages are whole numbers") from None
     except OverflowError:
-        a = array("I", [v & 0xFFFFFFFF for v in values])
-    return (C.c_uint32 * len(a)).from_buffer(a) if a else (C.c_uint32 * 1)()
+        pass
+    try:
+        return array("I", [_ffi.NO_PAGE if v == NO_PAGE else v for v in values])
+    except OverflowError:
+        raise ValueError("a page number does not fit") from None
 
 
-def _list(arr, lo: int, hi: int) -> List[int]:
-    out = arr[lo:hi]
-    return [NO_PAGE if v == _ffi.NO_PAGE else v for v in out] if _ffi.NO_PAGE in out else out
+def _addr(a) -> int:
+    return a.buffer_info()[0] if isinstance(a, array) else a.__array_interface__["data"][0]
 
 
 _IO: dict = {}           # torch dtype -> io_dtype, filled on first use (the package imports without torch)
@@ -130,41 +144,45 @@ class PagedKvCache:
 
     def alloc(self, n: int) -> List[int]:
         """The ``n`` lowest free pages; raises when fewer are free."""
-        out = (C.c_uint32 * max(n, 1))()
-        _ffi.check(_ffi.lib().vfkv_pages_alloc(self._h, n, out))
-        return list(out[:n])
+        out = np.empty(max(n, 1), np.uint32)
+        _ffi.check(_ffi.lib().vfkv_pages_alloc(self._h, n, _addr(out)))
+        return out[:n].tolist()
 
     def retain(self, pages: Sequence[int]) -> None:
-        _ffi.check(_ffi.lib().vfkv_pages_retain(self._h, _pages(pages), len(pages)))
+        p = _pages(pages)
+        _ffi.check(_ffi.lib().vfkv_pages_retain(self._h, _addr(p), len(p)))
 
     def release(self, pages: Sequence[int]) -> None:
         """One reference less per entry; pages without references are free (entries of -1 are skipped)."""
-        _ffi.check(_ffi.lib().vfkv_pages_release(self._h, _pages(pages), len(pages)))
+        p = _pages(pages)
+        _ffi.check(_ffi.lib().vfkv_pages_release(self._h, _addr(p), len(p)))
 
     # -- pages on the device --
     def copy_pages(self, src: Sequence[int], dst: Sequence[int], rows: Optional[Sequence[int]] = None, stream=None) -> None:
         """Copies page ``src[i]`` (its first ``rows[i]`` slots, default all) to page ``dst[i]``, all layers, K and V."""
-        if len(src) != len(dst) or (rows is not None and len(rows) != len(src)):
+        s, d, r = _pages(src), _pages(dst), None if rows is None else _pages(rows)
+        if len(s) != len(d) or (r is not None and len(r) != len(s)):
             raise ValueError("src, dst and rows must have the same length")
-        _ffi.check(_ffi.lib().vfkv_pages_copy(self._h, _pages(src), _pages(dst), None if rows is None else _pages(rows),
-                                              len(src), _stream(stream)))
+        _ffi.check(_ffi.lib().vfkv_pages_copy(self._h, _addr(s), _addr(d), None if r is None else _addr(r), len(s),
+                                              _stream(stream)))
 
-    def fork(self, pages: Sequence[int], kv_len: int, n_forks: int, stream=None) -> List[List[int]]:
-        """Page lists of ``n_forks`` continuations of the sequence of ``kv_len`` positions in ``pages``: full pages are
-        shared, a last page that is not full is copied into a page of the fork's own."""
+    def fork(self, pages: Sequence[int], kv_len: int, n_forks: int, stream=None) -> np.ndarray:
+        """Page lists [n_forks, pages] of continuations of the sequence of ``kv_len`` positions in ``pages``: full pages
+        are shared, a last page that is not full is copied into a page of the fork's own."""
         used = self.pages_for(kv_len)
-        if len(pages) < used:
-            raise ValueError(f"{kv_len} positions need {used} pages, got {len(pages)}")
-        out = (C.c_uint32 * max(used * n_forks, 1))()
-        _ffi.check(_ffi.lib().vfkv_pages_fork(self._h, _pages(pages[:used]), kv_len, n_forks, out,
+        p = _pages(pages)
+        if len(p) < used:
+            raise ValueError(f"{kv_len} positions need {used} pages, got {len(p)}")
+        out = np.empty((n_forks, used), np.int32)
+        _ffi.check(_ffi.lib().vfkv_pages_fork(self._h, _addr(p), kv_len, n_forks, _addr(out),
                                               _stream(stream) if self.k_ptr else None))
-        return [_list(out, i * used, (i + 1) * used) for i in range(n_forks)]
+        return out.astype(np.int64)
 
     def compact(self, stream=None) -> List[int]:
         """Moves the live pages into the lowest ids; returns every page's new id (-1: the page was free)."""
-        out = (C.c_uint32 * self.config.n_pages)()
-        _ffi.check(_ffi.lib().vfkv_pages_compact(self._h, out, _stream(stream) if self.k_ptr else None))
-        return _list(out, 0, self.config.n_pages)
+        out = np.empty(self.config.n_pages, np.int32)
+        _ffi.check(_ffi.lib().vfkv_pages_compact(self._h, _addr(out), _stream(stream) if self.k_ptr else None))
+        return out.tolist()
 
 
 def _int32(t, name: str):
