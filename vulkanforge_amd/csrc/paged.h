@@ -9,7 +9,7 @@
 
 namespace vfkv {
 
-constexpr uint32_t kPagedMaxLen = 1u << 30;   // positions of one sequence: sums with a tile's keys stay in 31 bits
+constexpr uint32_t kPagedMaxLen = 1u << 23;   // positions of one sequence: the 16-key units of a whole batch are counted in 32 bits
 
 struct PagedSlab {             // one layer
     const uint8_t* k;

@@ -41,6 +41,8 @@ struct DecShape {
     static constexpr int ES = DT == kF32 ? 4 : DT == kF16 ? 2 : 1;
     static constexpr int SUB = SUB_;                     // 16-key tiles per unit
     static constexpr int UK = 16 * SUB;                  // keys per unit
+    static constexpr int SHIFT = SUB == 1 ? 4 : SUB == 2 ? 5 : 6;
+    static_assert(UK == 1 << SHIFT, "units are powers of two");
     static constexpr int KE = 16 / ES;                   // elements of a 16-byte piece of a K row
     static constexpr int KL = D / (4 * KE);              // pieces per lane and row: piece x of lane group g is elements (4 x + g) KE ..
     static constexpr int NT = D / 16;                    // d-tiles = V elements per lane and key
@@ -54,15 +56,16 @@ struct DecShape {
 struct SeqUnits {
     uint32_t n, lo, sink, sink_units, first, units;
 };
-__device__ __forceinline__ SeqUnits seq_units(uint32_t n, uint32_t window, uint32_t n_sink, uint32_t uk) {
+__device__ __forceinline__ SeqUnits seq_units(uint32_t n, uint32_t window, uint32_t n_sink, uint32_t uk_shift) {
+    const uint32_t uk = 1u << uk_shift;
     SeqUnits r;
     r.n = n;
     r.lo = n ? paged_window_lo(window, n - 1u) : 0u;
     r.sink = n_sink < r.lo ? n_sink : r.lo;
-    r.first = r.lo / uk;
-    const uint32_t su = (r.sink + uk - 1u) / uk;
+    r.first = r.lo >> uk_shift;
+    const uint32_t su = (r.sink + uk - 1u) >> uk_shift;
     r.sink_units = su < r.first ? su : r.first;         // what reaches the window's first unit belongs to it
-    r.units = n ? r.sink_units + (n + uk - 1u) / uk - r.first : 0u;
+    r.units = n ? r.sink_units + ((n + uk - 1u) >> uk_shift) - r.first : 0u;
     return r;
 }
 
@@ -72,6 +75,10 @@ __device__ __forceinline__ uint32_t used_wgs(uint32_t U, uint32_t n_wg) {
     const uint32_t most = (U + kBegin + 2u * kDecWaves - 1u) / (kBegin + 2u * kDecWaves);
     return most < n_wg ? most : n_wg;
 }
+
+// floor(a / b) for a < 2^41, b < 2^32 through f64: a quotient that is not whole is at least 2^-41 of itself away from the next whole
+// number, the division rounds by 2^-53.  (The 64-bit integer division is some hundred instructions.)
+__device__ __forceinline__ uint32_t div_floor(uint64_t a, uint32_t b) { return (uint32_t)((double)a / (double)b); }
 
 __device__ __forceinline__ float max_over_groups(float x) {   // over lanes with the same lane & 15
     float y = x;
@@ -90,13 +97,13 @@ __device__ __forceinline__ float ror8_sum(float x) { return x + dpp_f<kDppRor8>(
 __device__ __forceinline__ uint32_t line_units(uint32_t units) { return units ? units + kBegin : 0u; }
 
 // Prefix sums of the line: pre[s] for s <= n_seqs, by the whole workgroup.
-template <int UK>
+template <int SHIFT>
 __device__ __forceinline__ void unit_prefix(const PagedAttnLaunch& a, uint32_t* pre, uint32_t* wave_sum, int tid) {
     const int lane = tid & 63, w = tid >> 6;
     uint32_t carry = 0u;
     for (uint32_t base = 0; base < a.s.n_seqs; base += 256u) {
         const uint32_t s = base + (uint32_t)tid;
-        uint32_t x = s < a.s.n_seqs ? line_units(seq_units(paged_kv_len(a.s, s), a.window, a.n_sink, UK).units) : 0u;
+        uint32_t x = s < a.s.n_seqs ? line_units(seq_units(paged_kv_len(a.s, s), a.window, a.n_sink, SHIFT).units) : 0u;
         const uint32_t mine = x;
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) {
@@ -146,17 +153,17 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_decode_kernel(Pag
     if (direct) {
         s_first = wg;
         s_end = wg + 1u;
-        u1 = line_units(seq_units(__builtin_amdgcn_readfirstlane(paged_kv_len(a.s, wg)), a.window, a.n_sink, Z::UK).units);
+        u1 = line_units(seq_units(__builtin_amdgcn_readfirstlane(paged_kv_len(a.s, wg)), a.window, a.n_sink, Z::SHIFT).units);
         if (u1 == 0u) { no_keys(wg); return; }
     } else {
-        unit_prefix<Z::UK>(a, pre, wave_sum, tid);
+        unit_prefix<Z::SHIFT>(a, pre, wave_sum, tid);
         const uint32_t U = pre[a.s.n_seqs];
         for (uint32_t s = wg; s < a.s.n_seqs; s += n_wg)
             if (pre[s + 1u] == pre[s]) no_keys(s);
         const uint32_t n_eff = used_wgs(U, n_wg);
         if (wg >= n_eff) return;
-        u0 = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)wg * U / n_eff));
-        u1 = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)(wg + 1u) * U / n_eff));
+        u0 = __builtin_amdgcn_readfirstlane(div_floor((uint64_t)wg * U, n_eff));
+        u1 = __builtin_amdgcn_readfirstlane(div_floor((uint64_t)(wg + 1u) * U, n_eff));
         uint32_t x = 0u, y = a.s.n_seqs - 1u;                            // the last s with pre[s] <= u0 (it has units)
         while (x < y) {
             const uint32_t mid = (x + y + 1u) >> 1;
@@ -195,7 +202,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_decode_kernel(Pag
         const uint32_t ps = direct ? 0u : __builtin_amdgcn_readfirstlane(pre[s]), pe = direct ? u1 : __builtin_amdgcn_readfirstlane(pre[s + 1u]);
         if (ps >= u1) break;
         if (ps == pe) continue;
-        const SeqUnits Q = seq_units(__builtin_amdgcn_readfirstlane(paged_kv_len(a.s, s)), a.window, a.n_sink, Z::UK);
+        const SeqUnits Q = seq_units(__builtin_amdgcn_readfirstlane(paged_kv_len(a.s, s)), a.window, a.n_sink, Z::SHIFT);
         // this range's part of the sequence, units [ua, ub)
         const uint32_t la = (ps > u0 ? ps : u0) - ps, lb = (pe < u1 ? pe : u1) - ps;
         const uint32_t ua = la > kBegin ? la - kBegin : 0u, ub = lb > kBegin ? lb - kBegin : 0u;
@@ -507,64 +514,93 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_decode_kernel(Pag
 
 // Joins the parts of the sequences that lie in more than one workgroup's range: one workgroup per (head, sequence).  The parts are
 // dealt to groups of D / 4 threads, each thread four columns.
-__global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnLaunch a, uint32_t n_wg, uint32_t uk) {
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnLaunch a, uint32_t n_wg, uint32_t uk_shift) {
     __shared__ uint32_t red[2][kDecWaves];
     __shared__ float4_t sums[256];
-    __shared__ float ls[256];
+    __shared__ float ls[256], ms[256];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const uint32_t head = blockIdx.x, s = blockIdx.y;
-    const uint32_t mine = line_units(seq_units(paged_kv_len(a.s, s), a.window, a.n_sink, uk).units);
-    uint32_t before = 0u, all = 0u;
-    for (uint32_t t = tid; t < a.s.n_seqs; t += 256u) {
-        const uint32_t x = line_units(seq_units(paged_kv_len(a.s, t), a.window, a.n_sink, uk).units);
-        all += x;
-        before += t < s ? x : 0u;
-    }
+    const uint32_t mine = line_units(seq_units(paged_kv_len(a.s, s), a.window, a.n_sink, uk_shift).units);
+    uint32_t before = 0u, U = mine;
+    if (a.s.n_seqs > 1u) {
+        uint32_t all = 0u;
+        for (uint32_t t = tid; t < a.s.n_seqs; t += 256u) {
+            const uint32_t x = line_units(seq_units(paged_kv_len(a.s, t), a.window, a.n_sink, uk_shift).units);
+            all += x;
+            before += t < s ? x : 0u;
+        }
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) {
-        before += __shfl_xor(before, off, kWave);
-        all += __shfl_xor(all, off, kWave);
+        for (int off = 32; off >= 1; off >>= 1) {
+            before += __shfl_xor(before, off, kWave);
+            all += __shfl_xor(all, off, kWave);
+        }
+        if (lane == 0) { red[0][w] = before; red[1][w] = all; }
+        __syncthreads();
+        before = red[0][0] + red[0][1] + red[0][2] + red[0][3];
+        U = red[1][0] + red[1][1] + red[1][2] + red[1][3];
     }
-    if (lane == 0) { red[0][w] = before; red[1][w] = all; }
-    __syncthreads();
-    before = red[0][0] + red[0][1] + red[0][2] + red[0][3];
-    const uint32_t U = red[1][0] + red[1][1] + red[1][2] + red[1][3];
     if (mine == 0u) return;
     // workgroup of unit u: the largest w with w U / N <= u
     n_wg = used_wgs(U, n_wg);
-    const uint32_t wa = (uint32_t)((((uint64_t)before + kBegin + 1u) * n_wg - 1u) / U);   // of its first unit
-    const uint32_t wb = (uint32_t)((((uint64_t)before + mine) * n_wg - 1u) / U);
+    const uint32_t wa = div_floor(((uint64_t)before + kBegin + 1u) * n_wg - 1u, U);   // of its first unit
+    const uint32_t wb = div_floor(((uint64_t)before + mine) * n_wg - 1u, U);
     if (wa == wb) return;                                                // written by the workgroup itself
     const uint32_t dr = a.c.head_dim, quads = dr / 4u;
     const uint32_t groups = 256u / quads, grp = (uint32_t)tid / quads, q4 = (uint32_t)tid % quads;
-    auto part_row = [&](uint32_t x) {
-        const bool first = (uint64_t)x * U / n_wg >= before;             // the sequence is the first of that range
-        return ((uint64_t)x * 2u + (first ? 0u : 1u)) * a.n_heads + head;
-    };
-    float M = kMasked;
-    for (uint32_t x = wa + (uint32_t)lane; x <= wb; x += 64u) M = fmaxf(M, a.scratch_max[part_row(x)]);
-    M = wave_max_all(M);
+    // (a range that begins inside the sequence, any but the first, has it as its first sequence)
+    const uint32_t slot_a = div_floor((uint64_t)wa * U, n_wg) >= before ? 0u : 1u;
+    auto part_row = [&](uint32_t x) { return ((uint64_t)x * 2u + (x == wa ? slot_a : 0u)) * a.n_heads + head; };
+    // eight parts at a time, maxima, sums and outputs requested together: one trip to memory for up to 8 * groups parts
+    constexpr int AT_ONCE = 8;
+    float M = kMasked, L = 0.f;
     float4_t sum = {0.f, 0.f, 0.f, 0.f};
-    float L = 0.f;
     if (grp < groups) {
-        for (uint32_t x = wa + grp; x <= wb; x += groups) {
-            const uint64_t row = part_row(x);
-            const float f = __builtin_amdgcn_exp2f(a.scratch_max[row] - M);
-            const float4_t v = *reinterpret_cast<const float4_t*>(a.scratch_out + row * dr + q4 * 4u);
-            L = __builtin_fmaf(a.scratch_sum[row], f, L);
+        for (uint32_t x0 = wa + grp; x0 <= wb; x0 += AT_ONCE * groups) {
+            float m[AT_ONCE], l[AT_ONCE];
+            float4_t v[AT_ONCE];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) sum[j] = __builtin_fmaf(v[j], f, sum[j]);
+            for (int i = 0; i < AT_ONCE; ++i) {
+                const uint32_t x = x0 + (uint32_t)i * groups;
+                const uint64_t row = part_row(x <= wb ? x : wb);
+                m[i] = a.scratch_max[row];
+                l[i] = a.scratch_sum[row];
+                v[i] = *reinterpret_cast<const float4_t*>(a.scratch_out + row * dr + q4 * 4u);
+            }
+            float mn = M;
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) mn = fmaxf(mn, m[i]);
+            const float old = __builtin_amdgcn_exp2f(M - mn);
+            M = mn;
+            L *= old;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sum[j] *= old;
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) {
+                if (x0 + (uint32_t)i * groups > wb) break;
+                const float f = __builtin_amdgcn_exp2f(m[i] - M);
+                L = __builtin_fmaf(l[i], f, L);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sum[j] = __builtin_fmaf(v[i][j], f, sum[j]);
+            }
         }
     }
     sums[tid] = sum;
     ls[tid] = L;
+    ms[tid] = M;
     __syncthreads();
     if (grp != 0u) return;
+    float top = M;
+    for (uint32_t x = 1; x < groups; ++x) top = fmaxf(top, ms[x * quads + q4]);
+    const float own = __builtin_amdgcn_exp2f(M - top);
+    L *= own;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum[j] *= own;
     for (uint32_t x = 1; x < groups; ++x) {
         const float4_t v = sums[x * quads + q4];
-        L += ls[x * quads + q4];
+        const float f = __builtin_amdgcn_exp2f(ms[x * quads + q4] - top);
+        L = __builtin_fmaf(ls[x * quads + q4], f, L);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sum[j] += v[j];
+        for (int j = 0; j < 4; ++j) sum[j] = __builtin_fmaf(v[j], f, sum[j]);
     }
     const float inv = L != 0.f ? 1.0f / L : 0.f;
     const uint64_t at = (uint64_t)s * a.o_stride + (uint64_t)head * dr + q4 * 4u;
@@ -607,7 +643,7 @@ hipError_t launch_dec(const PagedAttnLaunch& L, hipStream_t stream) {
     hipLaunchKernelGGL((paged_decode_kernel<DT, D, SUB>), dim3(n_hg, (uint32_t)n), dim3(256), (L.s.n_seqs + 1u) * 4u, stream, L, (uint32_t)n, slices, 0u);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || n == 1u) return e;
-    hipLaunchKernelGGL(paged_merge_kernel, dim3(L.n_heads, L.s.n_seqs), dim3(256), 0, stream, L, (uint32_t)n, UK);
+    hipLaunchKernelGGL(paged_merge_kernel, dim3(L.n_heads, L.s.n_seqs), dim3(256), 0, stream, L, (uint32_t)n, (uint32_t)DecShape<DT, D, SUB>::SHIFT);
     return hipGetLastError();
 }
 
