@@ -629,8 +629,10 @@ hipError_t launch_dec(const PagedAttnLaunch& L, hipStream_t stream) {
     uint64_t keys = L.max_kv;
     if (L.window != 0u && (uint64_t)L.window + L.n_sink + 2u * UK < keys) keys = (uint64_t)L.window + L.n_sink + 2u * UK;
     const uint64_t per_seq = (keys + UK - 1u) / UK;
-    // Short sequences (up to four units per wavefront): a workgroup each, without the prefix sums and without a join.
-    if (per_seq <= 4u * kDecWaves) {
+    // A workgroup per sequence, without the prefix sums and without a join: up to eight units per wavefront, up to sixteen when there
+    // are two workgroups per CU or more.  (FP8 heads of 128, 8 KV heads, dealt / a workgroup each: 64 sequences of 200-600 keys
+    // 25.5 / 15.8 us, one of 1 000 12.8 / 11.8, 64 of 1 000-2 000 51.1 / 45.1, 16 of 1 000-4 000 25.4 / 32.1.)
+    if (per_seq <= 8u * kDecWaves || (per_seq <= 16u * kDecWaves && (uint64_t)L.s.n_seqs * n_hg >= 512u)) {
         hipLaunchKernelGGL((paged_decode_kernel<DT, D, SUB>), dim3(n_hg, L.s.n_seqs), dim3(256), 0, stream, L, L.s.n_seqs, slices, 1u);
         return hipGetLastError();
     }
