@@ -540,9 +540,9 @@ hipError_t launch_pre(const PagedAttnLaunch& L, hipStream_t stream) {
     uint64_t blocks = L.s.n_tokens * group / R + with_rows;
     if (blocks > L.s.n_tokens * group) blocks = L.s.n_tokens * group;
     if (blocks > 65535u * 4096ull) return hipErrorInvalidValue;
-    // split over the keys: as long as the card has room, at least 128 keys per part (F32 pages: 32, a tile is longer work there
-    // than the join)
-    constexpr uint64_t least = DT == kF32 ? 32u : 128u;
+    // split over the keys: as long as the card has room, down to one tile per part (7 tokens over 1 000 keys, F16 heads of 64: parts of
+    // 64 / 256 keys 12.6 / 17.6 us; over F32 pages 32 / 256 keys 20.8 / 59.5 us)
+    constexpr uint64_t least = DT == kF32 ? 32u : 64u;
     const uint64_t likely = (L.s.n_tokens * group + R - 1u) / R * L.c.n_kv_heads;
     const uint64_t room = 256u * MINW * 4u / NW;
     uint64_t keys = L.max_kv;
