@@ -514,7 +514,8 @@ int vfkv_pages_release(vfkv_pages* c, const uint32_t* pages, uint32_t n);
 /* Copies the first rows[i] slots (rows NULL: all page_size) of page src[i] to page dst[i], all layers and heads, K and V, for
  * i < n.  src, dst and rows are HOST arrays, read before the call returns (a captured call replays the same copies).
  * Destinations must be distinct and none may be a source of the same call (VFKV_ERR_INVALID_ARG); reference counts
- * are neither checked nor changed. */
+ * are neither checked nor changed.  (vfkv_pages_fork and vfkv_pages_compact do their counting at the call, once: capture
+ * vfkv_pages_copy where the copies are to be replayed.) */
 int vfkv_pages_copy(vfkv_pages* c, const uint32_t* src, const uint32_t* dst, const uint32_t* rows, uint32_t n,
                     vfkv_stream stream);
 /* n_forks continuations of a sequence of kv_len positions whose ceil(kv_len / page_size) pages are `pages` (all live; entries
@@ -541,8 +542,9 @@ typedef struct vfkv_seq_batch {
     const int32_t* q_offsets;  /* [n_seqs + 1], not decreasing, or NULL: one token per sequence */
     uint32_t n_seqs;           /* <= 4096 */
     uint32_t table_stride;     /* page table entries per sequence */
-    uint32_t n_tokens;         /* rows of q / k / v / o */
-    uint32_t max_kv_len;       /* upper bound of kv_lens that sizes the launch (0: none known).  Results do not depend on it. */
+    uint32_t n_tokens;         /* rows of q / k / v / o, < 2^24 */
+    uint32_t max_kv_len;       /* upper bound of kv_lens that sizes the launch (0: none known).  Only the order of the sums depends on
+                                * it: lengths beyond it are followed all the same. */
 } vfkv_seq_batch;
 
 /* Norm, rotation and append of a batch: what vfkv_qk_rope_kv_write does for one sequence (executor/attention.rs:360-597), with
@@ -568,8 +570,9 @@ typedef struct vfkv_mrope_params {
  * into q_out (which may be q); k and v [n_tokens][n_kv_heads][head_dim] are appended at their tokens' positions, k
  * normalised and rotated first.  io_dtype (VFKV_F32 / VFKV_F16) is the type of q, k, v and q_out; *_stride the elements between two
  * tokens' rows (0: contiguous), so slices of one projection output need no copy.  positions [n_axes][n_tokens] int32 on the
- * device, NULL: every axis has the token's position in its sequence (one per token: n_axes rows of them otherwise).
- * freq_factors [rotary_dim / 2] f32 on the device or NULL.  Two sequences that share a page must not both append to it. */
+ * device, NULL: every axis has the token's position in its sequence.
+ * freq_factors [rotary_dim / 2] f32 on the device or NULL.  Two sequences that share a page must not both append to it: of two
+ * tokens that fall on the same slot either may stay, element by element (vfkv_pages_fork gives every fork a last page of its own). */
 typedef struct vfkv_paged_rows {
     const void* q;
     const float* q_norm_weight;
@@ -586,9 +589,14 @@ typedef struct vfkv_paged_rows {
 int vfkv_paged_qk_rope_kv_write(vfkv_pages* c, uint32_t layer, const vfkv_seq_batch* b, const vfkv_paged_rows* rows,
                                 const vfkv_mrope_params* p, vfkv_stream stream);
 
-/* What a query sees and how its scores are formed.  The query at position p sees key j when j <= p and
+/* Both attention calls run on the matrix cores for head_dim a multiple of 16 up to 256 with q and o 16-byte aligned and strides a
+ * multiple of 16 bytes; everything else takes a generic kernel (vfkv_last_note says so).  o must not overlap q.
+ *
+ * What a query sees and how its scores are formed.  The query at position p sees key j when j <= p and
  * (window == 0 or j > p - window or j < n_sink): a sliding window behind a few first tokens that stay visible.  A query
- * that sees nothing gets zeros. */
+ * that sees nothing gets zeros.  What a query does not see has no part in its output, whatever bits the rows hold (NaN, infinities);
+ * a row it does see enters by the formula, but an infinite element of K counts as NaN.  Over FP8 and F16 pages f32 queries enter the
+ * products as two f16 terms: |q| (prefill) and |q| * scale * 1.45 (decode) must stay below 65 504. */
 typedef struct vfkv_paged_attn_params {
     uint32_t n_heads;
     uint32_t window;   /* 0: all keys up to the query's own */
@@ -609,7 +617,7 @@ int vfkv_paged_workspace_create(const vfkv_pages* c, uint32_t n_heads, vfkv_work
 int vfkv_paged_decode_attention(vfkv_pages* c, uint32_t layer, const vfkv_seq_batch* b, const vfkv_paged_attn_params* p,
                                 const void* q, void* o, vfkv_workspace* ws, vfkv_stream stream);
 /* Any number of tokens per sequence, causal: chunks of prompts, drafted tokens, decode tokens among them.  ws may be NULL:
- * short chunks over long contexts then run without a split over the keys. */
+ * short chunks over long contexts then run without a split over the keys.  n_tokens * n_heads <= 2^30. */
 int vfkv_paged_prefill_attention(vfkv_pages* c, uint32_t layer, const vfkv_seq_batch* b, const vfkv_paged_attn_params* p,
                                  const void* q, void* o, vfkv_workspace* ws, vfkv_stream stream);
 

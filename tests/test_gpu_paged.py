@@ -606,3 +606,161 @@ def test_two_streams_with_workspaces_of_their_own():
     for i in range(2):
         ref, tol = attention(pools[i], qs[i], [1, 1])
         assert (outs[i].cpu().double() - ref).abs().max() <= tol
+
+
+@IOS
+def test_prefill_captured_follows_its_arrays(io):
+    """One captured prefill call, replayed with other lengths, offsets and page tables, against the eager call."""
+    pool = Pool(F8, 2, 128, 16, [200, 90, 33], spare=0)
+    fwd = vf.PagedForward(pool.cache, 8)
+    n = 60
+    off = torch.tensor([0, 20, 21, 55], dtype=torch.int32, device=DEV)
+    kv, table = pool.kv_dev.clone(), pool.table_dev.clone()
+    batch = vf.SeqBatch(table, kv, off, n_tokens=n)
+    q = rand_q(n, 8, 128, io)
+    o = torch.zeros_like(q)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        fwd.prefill_attention(0, batch, q, o, window=70, n_sink=5)
+    for rep, (lens, offsets) in enumerate((([200, 90, 33], [0, 20, 21, 55]), ([20, 90, 0], [0, 5, 40, 40]), ([199, 1, 33], [0, 0, 1, 34]),
+                                           ([200, 64, 32], [0, 30, 59, 60]))):
+        kv.copy_(torch.tensor(lens, dtype=torch.int32))
+        off.copy_(torch.tensor(offsets, dtype=torch.int32))
+        q.copy_(rand_q(n, 8, 128, io, seed=rep))
+        o.fill_(7.0)
+        graph.replay()
+        eager = torch.full_like(o, 7.0)
+        fwd.prefill_attention(0, batch, q, eager, window=70, n_sink=5)
+        torch.cuda.synchronize()
+        assert torch.equal(o, eager) and bool((o[offsets[-1]:] == 7.0).all()) and bool(o.isfinite().all())
+        (q * 2).sum().item()
+
+
+def test_decode_4096_sequences():
+    kv = [(13 * i) % 37 for i in range(4096)]
+    pool = Pool(F16, 1, 16, 16, kv)
+    fwd = vf.PagedForward(pool.cache, 2)
+    q = rand_q(4096, 2, 16)
+    for bound in (36, 0, 5000):                            # a workgroup per sequence; dealt
+        o = torch.full_like(q, float("nan"))
+        fwd.decode_attention(0, vf.SeqBatch(pool.table_dev, pool.kv_dev, max_kv_len=bound), q, o)
+        torch.cuda.synchronize()
+        assert bool(o.isfinite().all())
+        for s in (0, 1, 5, 37, 2047, 4094, 4095):
+            one = Pool.__new__(Pool)
+            one.__dict__.update(pool.__dict__)
+            one.kv, one.table = [kv[s]], pool.table[s:s + 1]
+            ref, tol = attention(one, q[s:s + 1], [1])
+            assert (o[s:s + 1].cpu().double() - ref).abs().max() <= tol, s
+    wide = torch.zeros((4097, 1), dtype=torch.int32, device=DEV)
+    with pytest.raises(vf.VfkvError) as e:
+        fwd.decode_attention(0, vf.SeqBatch(wide, torch.zeros(4097, dtype=torch.int32, device=DEV)), rand_q(4097, 2, 16), rand_q(4097, 2, 16, seed=2))
+    assert e.value.status == -4
+
+
+@pytest.mark.parametrize("dtype, d, unit", [(F8, 128, 32), (F8, 64, 64), (F16, 64, 32), (F16, 256, 16), (F32, 128, 16), (F8, 256, 32)])
+def test_decode_lengths_around_the_ways_of_dealing(dtype, d, unit):
+    for kv in ([32 * unit - 1], [32 * unit], [32 * unit + 1], [33 * unit, 1, 40 * unit + 3, 0, unit], [unit, unit + 1, unit - 1, 1]):
+        pool = Pool(dtype, 2, d, 64, kv)
+        check_attention(pool, 4, [1] * len(kv), decode=True)
+        check_attention(pool, 4, [1] * len(kv), decode=True, max_kv_len=1)      # a bound that does not hold: slower, not wrong
+
+
+def test_write_many_sequences_and_offsets():
+    n = 150                                                   # more sequences than lanes
+    q_len = [(7 * i) % 4 for i in range(n)]
+    kv = [m + (11 * i) % 29 for i, m in enumerate(q_len)]
+    write_case(F8, torch.float32, 4, 2, 64, 16, q_len, kv, 64, vf.ROPE_NEOX, [32], False)
+    write_case(F16, torch.float16, 2, 1, 33, 16, q_len, kv, 32, vf.ROPE_NORM, [8, 8], True)
+
+
+def test_sequences_may_share_pages():
+    pool = Pool(F16, 2, 64, 16, [64, 80])
+    pool.table[1, :4] = pool.table[0, :4]
+    pool.table_dev.copy_(pool.table)
+    check_attention(pool, 4, [1, 1], decode=True)
+    check_attention(pool, 4, [30, 40])
+
+
+@DTYPES
+@IOS
+def test_values_of_later_tokens_do_not_reach_earlier_ones(dtype, io):
+    """Infinities and NaN in V rows of the chunk itself: the rows that see them get them, the earlier ones are untouched."""
+    bad = float("nan") if dtype == F8 else float("inf")
+    for hq, m, window in ((2, 70, 0), (8, 40, 0), (2, 70, 20), (1, 300, 33)):
+        pool = Pool(dtype, 1, 128, 16, [m + 30])
+        at = m + 10                                           # a key in the middle of the chunk
+        p, sl = int(pool.table[0, at // 16]), at % 16
+        clean = Pool(dtype, 1, 128, 16, [m + 30])
+        row = pool.v[0, p, 0, sl].float().clone()
+        row[5] = bad
+        pool.v[0, p, 0, sl] = row.to(pool.v.dtype)
+        fwd = [vf.PagedForward(x.cache, hq) for x in (pool, clean)]
+        q = rand_q(m, hq, 128, io)
+        o = [torch.zeros_like(q) for _ in range(2)]
+        for f, x, y in zip(fwd, (pool, clean), o):
+            f.prefill_attention(0, x.batch([m]), q, y, window=window)
+        torch.cuda.synchronize()
+        pos = torch.arange(30, m + 30, device=DEV)
+        sees = (pos >= at) & ((pos - window < at) if window else True)
+        assert bool(sees.any()) and not bool(sees.all())
+        hit = ~o[0].isfinite()
+        assert bool(hit[sees][:, :, 5].all()) and not bool(hit[~sees].any()) and not bool(hit[..., :5].any()) and not bool(hit[..., 6:].any())
+        same = o[0].clone()
+        same[..., 5] = o[1][..., 5] = 0
+        assert torch.equal(same, o[1])
+
+
+def test_batch_on_another_device_is_refused():
+    pool = Pool(F16, 1, 64, 16, [5])
+    fwd = vf.PagedForward(pool.cache, 2)
+    pool.cache.device = 1                                     # as if the cache were there
+    with pytest.raises(ValueError):
+        fwd.decode_attention(0, pool.batch(), rand_q(1, 2, 64), rand_q(1, 2, 64, seed=2))
+    with pytest.raises(ValueError):
+        fwd.qk_rope_kv_write(0, pool.batch(), None, rand_q(1, 1, 64), rand_q(1, 1, 64), vf.MRope(0))
+
+
+def test_prefill_without_a_workspace():
+    import ctypes as C
+    from vulkanforge_amd import _ffi
+    pool = Pool(F8, 2, 128, 16, [3000])
+    q = rand_q(5, 8, 128)
+    o = torch.empty_like(q)
+    b = pool.batch([5])
+    p = _ffi.PagedAttnParams(8, 0, 0, 0, 0, 0, 1.0 / math.sqrt(128), 0.0)
+    _ffi.check(_ffi.lib().vfkv_paged_prefill_attention(pool.cache.handle, 0, b.args, C.byref(p), q.data_ptr(), o.data_ptr(), None,
+                                                       torch.cuda.current_stream().cuda_stream))
+    torch.cuda.synchronize()
+    ref, tol = attention(pool, q, [5])
+    assert (o.cpu().double() - ref).abs().max() <= tol
+
+
+def test_a_small_workspace_only_limits_the_split():
+    pool = Pool(F8, 2, 128, 16, [5000, 40])
+    for max_seq in (1, 64, 256, 100000):
+        ws = vf.Workspace(8, 128, max_seq)
+        ws.handle = ws._h
+        fwd = vf.PagedForward(pool.cache, 8, workspace=ws)
+        for q_len in (None, [9, 3]):
+            n = 2 if q_len is None else 12
+            q = rand_q(n, 8, 128)
+            o = torch.full_like(q, float("nan"))
+            (fwd.decode_attention if q_len is None else fwd.prefill_attention)(0, pool.batch(q_len), q, o)
+            torch.cuda.synchronize()
+            ref, tol = attention(pool, q, q_len or [1, 1])
+            assert (o.cpu().double() - ref).abs().max() <= tol
+
+
+def test_generic_kernel_leaves_a_note():
+    from vulkanforge_amd import _ffi
+    note = lambda: _ffi.lib().vfkv_last_note()  # noqa: E731
+    for d, text in ((64, b""), (72, b"generic")):
+        pool = Pool(F16, 1, d, 16, [20])
+        fwd = vf.PagedForward(pool.cache, 2)
+        q = rand_q(1, 2, d)
+        for call in (fwd.decode_attention, ):
+            call(0, pool.batch(), q, torch.empty_like(q))
+            assert (text in note()) if text else note() == b""
+    torch.cuda.synchronize()

@@ -72,7 +72,7 @@ int check_batch(const vfkv_pages* c, const vfkv_seq_batch* b, const char* who, v
         return fail(VFKV_ERR_ALIGNMENT, "%s: the batch's arrays must be 4-byte aligned", who);
     if (b->n_seqs > vfkv::kPagedMaxSeqs) return fail(VFKV_ERR_UNSUPPORTED, "%s: %u sequences (at most %u in one call)", who, b->n_seqs, vfkv::kPagedMaxSeqs);
     if (b->table_stride == 0u) return fail(VFKV_ERR_INVALID_ARG, "%s: table_stride must be > 0", who);
-    if (b->n_tokens > 0x7FFFFFFFu) return fail(VFKV_ERR_UNSUPPORTED, "%s: %u tokens", who, b->n_tokens);
+    if (b->n_tokens >= 1u << 24) return fail(VFKV_ERR_UNSUPPORTED, "%s: %u tokens (less than 2^24 in one call)", who, b->n_tokens);
     if (!b->q_offsets && b->n_tokens != b->n_seqs)
         return fail(VFKV_ERR_INVALID_ARG, "%s: without q_offsets every sequence has one token (%u tokens, %u sequences)", who, b->n_tokens, b->n_seqs);
     const uint64_t held = (uint64_t)b->table_stride << c->page_shift;
@@ -178,7 +178,19 @@ int vfkv_pages_create_external(const vfkv_pages_config* cfg, void* k_buffer, voi
             delete c;
             throw;
         }
-        if (k_buffer && hipGetDevice(&c->device) != hipSuccess) c->device = -1;   // (no device: every compute call fails later)
+        if (k_buffer) {
+            if (hipGetDevice(&c->device) != hipSuccess) c->device = -1;           // (no device: every compute call fails later)
+            for (void* p : {k_buffer, v_buffer}) {
+                hipPointerAttribute_t at;
+                if (hipPointerGetAttributes(&at, p) != hipSuccess) {
+                    (void)hipGetLastError();                                      // not a pointer the runtime knows: nothing to compare
+                } else if (at.type == hipMemoryTypeDevice && at.device != c->device) {
+                    const int there = at.device, here = c->device;
+                    delete c;
+                    return fail(VFKV_ERR_INVALID_ARG, "pages: a buffer is on device %d, the current device is %d", there, here);
+                }
+            }
+        }
         *out = c;
         return VFKV_OK;
     });
@@ -460,7 +472,7 @@ static int paged_attention(vfkv_pages* c, uint32_t layer, const vfkv_seq_batch* 
     if (q == o) return fail(VFKV_ERR_INVALID_ARG, "%s: o must not overlap q", who);
     if ((((uintptr_t)q | (uintptr_t)o) & (p->io_dtype == VFKV_F32 ? 3u : 1u)) != 0u)
         return fail(VFKV_ERR_ALIGNMENT, "%s: a buffer is not aligned to its element size", who);
-    if ((uint64_t)b->n_tokens * p->n_heads > 0xFFFFFFFFull) return fail(VFKV_ERR_OVERFLOW, "%s: n_tokens * n_heads exceeds 2^32 - 1", who);
+    if ((uint64_t)b->n_tokens * p->n_heads > 1u << 30) return fail(VFKV_ERR_UNSUPPORTED, "%s: n_tokens * n_heads exceeds 2^30", who);
     if (ws && (ws->n_heads < p->n_heads || ws->head_dim < hd))
         return fail(VFKV_ERR_WORKSPACE, "%s: workspace built for %u heads x %u dims, need %u x %u", who, ws->n_heads, ws->head_dim, p->n_heads, hd);
     if (decode && !ws) return fail(VFKV_ERR_INVALID_ARG, "%s: workspace is NULL", who);

@@ -111,15 +111,16 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
     const int tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n32 = lane & 31, hf = lane >> 5;
-    const uint32_t group = a.n_heads / a.c.n_kv_heads, kvh = blockIdx.x;
+    // KV head fastest: consecutive workgroups go to different XCDs, so with eight heads each XCD keeps one head's keys in its L2
+    const uint32_t group = a.n_heads / a.c.n_kv_heads, block = blockIdx.x / a.c.n_kv_heads, kvh = blockIdx.x - block * a.c.n_kv_heads;
     const uint32_t dr = a.c.head_dim;
     uint32_t* const pre = reinterpret_cast<uint32_t*>(lds);
     static_assert(2 * Z::BUF >= ((int)kPagedMaxSeqs + 1) * 4, "the prefix sums fit the tile buffers");
     if (tid == 0) n_odd = 0u;
     block_prefix<NW>(a, group, R, pre, wave_sum, tid);
     const uint32_t blocks = __builtin_amdgcn_readfirstlane(pre[a.s.n_seqs]);
-    if (blockIdx.y >= blocks) return;
-    const uint32_t bi = blocks - 1u - blockIdx.y;
+    if (block >= blocks) return;
+    const uint32_t bi = blocks - 1u - block;
     uint32_t s;
     {
         uint32_t x = 0u, y = a.s.n_seqs - 1u;                // the last s with pre[s] <= bi
@@ -133,7 +134,7 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
     paged_rows(a.s, s, t0, t1);
     t0 = __builtin_amdgcn_readfirstlane(t0);
     t1 = __builtin_amdgcn_readfirstlane(t1);
-    const uint32_t n_rows = (t1 - t0) * group;               // (< 2^31 * 2^16 would not fit: the launcher refuses n_tokens * n_heads >= 2^32)
+    const uint32_t n_rows = (t1 - t0) * group;               // (n_tokens * n_heads <= 2^30)
     const uint32_t row0 = (bi - __builtin_amdgcn_readfirstlane(pre[s])) * R;
     __syncthreads();                                         // the prefix sums have been read: the buffers are free
     const uint32_t row1 = n_rows - row0 < R ? n_rows : row0 + R;
@@ -148,7 +149,7 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
     const uint32_t su = (sink + KT - 1u) / KT;
     const uint32_t sink_tiles = su < first ? su : first;
     const uint32_t tiles = n_keys ? sink_tiles + (n_keys + KT - 1u) / KT - first : 0u;
-    const uint32_t ta = (uint32_t)((uint64_t)blockIdx.z * tiles / n_split), tb = (uint32_t)((uint64_t)(blockIdx.z + 1u) * tiles / n_split);
+    const uint32_t ta = (uint32_t)((uint64_t)blockIdx.y * tiles / n_split), tb = (uint32_t)((uint64_t)(blockIdx.y + 1u) * tiles / n_split);
     auto tile_key = [&](uint32_t t) { return (t < sink_tiles ? t : first + t - sink_tiles) * (uint32_t)KT; };
 
     // ---- this wavefront's rows
@@ -479,7 +480,7 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
 
     // ---- output
     const float L = xor32_sum(l);
-    const uint64_t row = ((uint64_t)tok * a.n_heads + head) * n_split + blockIdx.z;
+    const uint64_t row = ((uint64_t)tok * a.n_heads + head) * n_split + blockIdx.y;
     const uint64_t at = (uint64_t)tok * a.o_stride + (uint64_t)head * dr;
     if (real) {
         const float inv = n_split > 1u ? 1.0f : L != 0.f ? 1.0f / L : 0.f;
@@ -539,7 +540,7 @@ hipError_t launch_pre(const PagedAttnLaunch& L, hipStream_t stream) {
     const uint64_t with_rows = L.s.n_seqs < L.s.n_tokens ? L.s.n_seqs : L.s.n_tokens;
     uint64_t blocks = L.s.n_tokens * group / R + with_rows;
     if (blocks > L.s.n_tokens * group) blocks = L.s.n_tokens * group;
-    if (blocks > 65535u * 4096ull) return hipErrorInvalidValue;
+    if (blocks * L.c.n_kv_heads * NW * 64u > 0xFFFFFFFFull) return hipErrorInvalidValue;   // (not with n_tokens * n_heads <= 2^30)
     // split over the keys: as long as the card has room, down to one tile per part (7 tokens over 1 000 keys, F16 heads of 64: parts of
     // 64 / 256 keys 12.6 / 17.6 us; over F32 pages 32 / 256 keys 20.8 / 59.5 us)
     constexpr uint64_t least = DT == kF32 ? 32u : 64u;
@@ -553,7 +554,7 @@ hipError_t launch_pre(const PagedAttnLaunch& L, hipStream_t stream) {
     if (n > fits) n = fits;
     if (n > 64u) n = 64u;
     if (n == 0u) n = 1u;
-    hipLaunchKernelGGL((paged_prefill_kernel<DT, D, IOF16, CAP, KT, CK, NW, MINW>), dim3(L.c.n_kv_heads, (uint32_t)blocks, (uint32_t)n), dim3(NW * 64),
+    hipLaunchKernelGGL((paged_prefill_kernel<DT, D, IOF16, CAP, KT, CK, NW, MINW>), dim3((uint32_t)(blocks * L.c.n_kv_heads), (uint32_t)n), dim3(NW * 64),
                        2u * Z::BUF, stream, L, (uint32_t)n);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || n == 1u) return e;

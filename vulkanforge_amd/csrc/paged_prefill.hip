@@ -97,7 +97,7 @@ hipError_t launch_paged_rows_merge(const PagedAttnLaunch& L, uint32_t n_split, h
 }
 
 hipError_t launch_paged_prefill(const PagedAttnLaunch& L, hipStream_t stream) {
-    if ((uint64_t)L.s.n_tokens * L.n_heads > 0xFFFFFFFFull) return hipErrorInvalidValue;
+    if ((uint64_t)L.s.n_tokens * L.n_heads > 1u << 30) return hipErrorInvalidValue;
     if (L.c.dtype == kF8) return launch_paged_prefill_byte(L, stream);
     return L.c.dtype == kF16 ? launch_paged_prefill_half(L, stream) : launch_paged_prefill_full(L, stream);
 }

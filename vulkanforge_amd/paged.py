@@ -99,6 +99,14 @@ class PagedKvCache:
         else:
             _ffi.check(L.vfkv_pages_create(C.byref(cfg), C.byref(handle)))
         self._h = handle
+        self.device = None                               # index of the device the buffers are on
+        if self.k_ptr:
+            try:
+                import torch
+                if torch.cuda.is_available():
+                    self.device = torch.cuda.current_device()
+            except ImportError:
+                pass
 
     def destroy(self) -> None:
         if getattr(self, "_h", None):
@@ -207,6 +215,8 @@ class SeqBatch:
             if q_offsets is not None:
                 raise ValueError("n_tokens is needed with q_offsets (the offsets are on the device)")
             n_tokens = n
+        if n_tokens < 0 or not 0 <= max_kv_len <= 0xFFFFFFFF:
+            raise ValueError("n_tokens and max_kv_len must not be negative")
         devices = {t.device for t in (page_table, kv_lens, q_offsets) if t is not None}
         if len(devices) != 1:
             raise ValueError("page_table, kv_lens and q_offsets must be on one device")
@@ -264,6 +274,8 @@ class PagedForward:
     def _rows(self, t, heads: int, batch: SeqBatch, name: str):
         """(address, elements between two tokens, io dtype) of a row tensor."""
         dim = self.head_dim
+        if batch.index != self.cache.device:
+            raise ValueError(f"the batch is on {batch.device}, the cache on device {self.cache.device}")
         io = _IO.get(t.dtype)
         if io is None or t.get_device() != batch.index or t.shape != (batch.n_tokens, heads, dim):
             if not _IO:
