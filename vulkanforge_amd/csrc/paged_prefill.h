@@ -531,6 +531,12 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
 
 namespace {
 
+// Whether the blocks of a chunk see about as many keys each: a context in front of it, or a window that is short against it.
+bool blocks_alike(const PagedAttnLaunch& L) {
+    const uint64_t chunk = (L.s.n_tokens + L.s.n_seqs - 1u) / L.s.n_seqs;
+    return L.max_kv >= 2u * chunk || (L.window != 0u && chunk >= 2u * (uint64_t)L.window);
+}
+
 template <int DT, int D, bool IOF16, bool CAP, int KT, int CK, int NW, int MINW>
 hipError_t launch_pre(const PagedAttnLaunch& L, hipStream_t stream) {
     using Z = PreShape<DT, D, KT, NW>;
@@ -541,19 +547,26 @@ hipError_t launch_pre(const PagedAttnLaunch& L, hipStream_t stream) {
     uint64_t blocks = L.s.n_tokens * group / R + with_rows;
     if (blocks > L.s.n_tokens * group) blocks = L.s.n_tokens * group;
     if (blocks * L.c.n_kv_heads * NW * 64u > 0xFFFFFFFFull) return hipErrorInvalidValue;   // (not with n_tokens * n_heads <= 2^30)
-    // split over the keys: as long as the card has room, down to one tile per part (7 tokens over 1 000 keys, F16 heads of 64: parts of
-    // 64 / 256 keys 12.6 / 17.6 us; over F32 pages 32 / 256 keys 20.8 / 59.5 us)
-    constexpr uint64_t least = DT == kF32 ? 32u : 64u;
+    // Split over the keys, as long as the card has room and a part has a tile: the tiles of a part against the join, which writes and
+    // reads the parts once (about 4 TB/s and 3 us).  A tile takes about 2.2 us for f16 rows of 128 elements, 1.6 times that with
+    // value + remainder, 6.8 us for 32 keys on the f32 instruction.  (FP8, 32 / 8 / 128, one part against two: 1 024 f16 tokens from
+    // position 0 33.6 / 39.5 us, over 5 000 keys 162 / 104 us; 7 tokens over 1 000 keys, F16 heads of 64, 4 / 16 parts 17.6 / 12.6 us.)
+    constexpr uint64_t tile_ns = (DT == kF32 ? 6800u * KT / 32u : (IOF16 ? 2200u : 3500u) * KT / 64u) * D / 128u;
     const uint64_t likely = (L.s.n_tokens * group + R - 1u) / R * L.c.n_kv_heads;
-    const uint64_t room = 256u * MINW * 4u / NW;
+    // (unlike blocks: twice the workgroups that fit, so that the last ones are short; F16 rows of 256, 2 048 tokens 129 -> 105 us)
+    const uint64_t room = 256u * MINW * 4u / NW * (blocks_alike(L) ? 1u : 2u);
     uint64_t keys = L.max_kv;
     if (L.window != 0u && (uint64_t)L.window + L.n_sink + R + 2u * KT < keys) keys = (uint64_t)L.window + L.n_sink + R + 2u * KT;
-    uint64_t n = room / likely;
-    if (n > keys / least) n = keys / least;
-    const uint64_t fits = L.scratch_rows / ((uint64_t)L.s.n_tokens * L.n_heads);
-    if (n > fits) n = fits;
-    if (n > 64u) n = 64u;
-    if (n == 0u) n = 1u;
+    const uint64_t tiles = (keys + KT - 1u) / KT, rows = (uint64_t)L.s.n_tokens * L.n_heads;
+    uint64_t most = room / likely;
+    if (most > tiles) most = tiles;
+    if (most > L.scratch_rows / rows) most = L.scratch_rows / rows;
+    if (most > 64u) most = 64u;
+    uint64_t n = 1u, best = tiles * tile_ns;
+    for (uint64_t i = 2u; i <= most; ++i) {
+        const uint64_t ns = (tiles + i - 1u) / i * tile_ns + 3000u + rows * i * L.c.head_dim * 8u / 4000u;
+        if (ns < best) { best = ns; n = i; }
+    }
     hipLaunchKernelGGL((paged_prefill_kernel<DT, D, IOF16, CAP, KT, CK, NW, MINW>), dim3((uint32_t)(blocks * L.c.n_kv_heads), (uint32_t)n), dim3(NW * 64),
                        2u * Z::BUF, stream, L, (uint32_t)n);
     hipError_t e = hipGetLastError();
@@ -569,10 +582,18 @@ hipError_t launch_dim(const PagedAttnLaunch& L, hipStream_t stream) {
         if (d <= 128u) return launch_pre<DT, 128, IOF16, CAP, 32, 32, 4, 2>(L, stream);
         return launch_pre<DT, 256, IOF16, CAP, 32, 32, 4, 1>(L, stream);
     } else {
-        const bool many = (uint64_t)L.s.n_tokens * (L.n_heads / L.c.n_kv_heads) >= 256ull * L.s.n_seqs;
+        // Workgroups of eight wavefronts share a staged tile among twice the rows, but a card that they fill only once waits for the
+        // block with the most keys: they are taken for chunks that fill blocks of 256 rows, with two rounds of blocks or with a
+        // context that makes the blocks alike.  (FP8 / f16 rows of 128, eight / four wavefronts: 4 096 tokens from position 0
+        // 160 / 172 us, 2 048 76 / 65 us, 1 024 tokens over 5 000 keys 102 / 110 us; F16 rows of 256: 8 192 tokens 753 / 1 012 us,
+        // 4 096 327 / 271 us, 2 048 over 6 000 keys 301 / 356 us.)
+        const uint64_t rows = (uint64_t)L.s.n_tokens * (L.n_heads / L.c.n_kv_heads);
+        const bool many = rows >= 256ull * L.s.n_seqs && (blocks_alike(L) || rows / 256u * L.c.n_kv_heads >= 512u);
         constexpr int CK = IOF16 ? 64 : 32, KT = 64;
         if (d <= 64u) return many ? launch_pre<DT, 64, IOF16, CAP, 64, 64, 8, 2>(L, stream) : launch_pre<DT, 64, IOF16, CAP, 64, 64, 4, 2>(L, stream);
         if (d <= 128u) return many ? launch_pre<DT, 128, IOF16, CAP, KT, CK, 8, 2>(L, stream) : launch_pre<DT, 128, IOF16, CAP, KT, CK, 4, 2>(L, stream);
+        if constexpr (IOF16)                                     // (value + remainder of 256 elements do not fit 256 registers)
+            if (many) return launch_pre<DT, 256, IOF16, CAP, 32, 32, 8, 2>(L, stream);
         return launch_pre<DT, 256, IOF16, CAP, 32, 32, 4, 1>(L, stream);
     }
 }
