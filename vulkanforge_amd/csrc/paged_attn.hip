@@ -1,4 +1,4 @@
-// Attention over the paged cache.
+// Attention over the paged cache: the generic form.  (paged_decode.hip and paged_prefill.h hold the matrix-core kernels.)
 #include "device_utils.h"
 #include "paged.h"
 

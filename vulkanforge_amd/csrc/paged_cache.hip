@@ -10,7 +10,8 @@ namespace vfkv {
 // dst page <- src page for all layers, K and V: pure traffic, one read and one write per byte.  The pairs travel as kernel
 // arguments: no upload, and a captured call keeps its own list.  blockIdx.y = pair, blockIdx.z = layer and tensor, blockIdx.x =
 // share of the page.  A page of one layer is contiguous; with fewer rows it is n_kv_heads pieces, each at a multiple of
-// page_size rows, hence 16-byte aligned whatever the row length.
+// page_size rows, hence 16-byte aligned whatever the row length.  Measured: 200 pages of 128 KiB in 32 layers (3.36 GB read and written)
+// 632 us = 5.3 TB/s, what a copy of 1 GiB reaches (5.2); four partial pages (fork) 3.8 us.
 struct CopyArgs {
     uint8_t* buf[2];
     uint64_t layer_bytes, page_bytes;
@@ -124,6 +125,9 @@ __device__ __forceinline__ float4_t load_quad(const void* p, uint64_t i) {
 // rotated part holds both elements of its four pairs (quads p and p + rotary_dim / 2 apart, or eight neighbours), so nothing
 // crosses lanes but the sum of squares; the pairs' cos and sin are computed once per token and wavefront, one per lane, and passed
 // round.  A wavefront takes every `parts`-th group of rows of its token and requests kAhead of them before it works on the first.
+// Measured: 5 692 tokens, 32 / 8 / 128, f16 rows into F16 pages 36.5 us = 3.8 TB/s (element by element: 142 us; two or four steps
+// ahead and two to three wavefronts per token measured the same or slower: the vector units are busy half the time, a token's chain of
+// steps the other half); 32 decode tokens 5.8 us.
 constexpr int kAhead = 3;
 template <typename T, int LPR>
 __global__ __launch_bounds__(kWriteWaves * kWave) void paged_write_quads_kernel(PagedWriteLaunch a, uint32_t parts) {

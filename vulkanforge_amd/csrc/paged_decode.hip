@@ -20,6 +20,10 @@
 //         A = V^T: a lane loads D / 16 columns of its four keys per tile and turns that small matrix with byte permutes
 //         in its own registers -- no LDS, no barrier.
 //     F32 caches use the f32 matrix instruction with the same ownership; nothing needs turning there.
+// Measured, one layer (copy rate of the card: 5.2 TB/s): 48 sequences of 17-8 193 keys, FP8, 32 / 8 / 128: 80.6 us = 4.8 TB/s; 12 windows
+// of 4 096 keys, F16, 16 / 8 / 256, soft-capped: 82.4 us = 4.6 TB/s; one sequence of 65 536 keys: 25.8 us for the worker (5.2 TB/s) and
+// 6.0 us for the join; one of 200 keys 6.5 us (the chain length -> page -> rows -> join of the wavefronts).
+//
 //   - The running maximum is only raised when a score exceeds it by 2^8: weights are kept times 2^6 (at most 2^14 in f16, smallest
 //     step 2^-30 of the largest), and the accumulators are rescaled a few times per sequence instead of once per unit.
 #include "device_utils.h"
@@ -513,7 +517,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_decode_kernel(Pag
 }
 
 // Joins the parts of the sequences that lie in more than one workgroup's range: one workgroup per (head, sequence).  The parts are
-// dealt to groups of D / 4 threads, each thread four columns.
+// dealt to groups of D / 4 threads, each thread four columns.  Latency bound: 6.0 us for one sequence in 64 parts.
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnLaunch a, uint32_t n_wg, uint32_t uk_shift) {
     __shared__ uint32_t red[2][kDecWaves];
     __shared__ float4_t sums[256];
