@@ -498,7 +498,7 @@ void* vfkv_pages_v_ptr(const vfkv_pages* c);
 uint64_t vfkv_pages_bytes_per_buffer(const vfkv_pages* c);
 uint64_t vfkv_pages_offset_bytes(const vfkv_pages* c, uint32_t layer, uint32_t page); /* start of a page in either buffer */
 
-/* Page counting (host only, immediate).  Calls on one object must not overlap in time. */
+/* Page counting (host only, immediate).  Calls on one object, those below that move pages included, must not overlap in time. */
 uint32_t vfkv_pages_free_count(const vfkv_pages* c);
 uint32_t vfkv_pages_refcount(const vfkv_pages* c, uint32_t page); /* 0 = free (or out of range) */
 /* The n lowest free pages, in ascending order, one reference each.  VFKV_ERR_WORKSPACE when fewer are free; nothing is
@@ -595,8 +595,9 @@ int vfkv_paged_qk_rope_kv_write(vfkv_pages* c, uint32_t layer, const vfkv_seq_ba
  * What a query sees and how its scores are formed.  The query at position p sees key j when j <= p and
  * (window == 0 or j > p - window or j < n_sink): a sliding window behind a few first tokens that stay visible.  A query
  * that sees nothing gets zeros.  What a query does not see has no part in its output, whatever bits the rows hold (NaN, infinities);
- * a row it does see enters by the formula, but an infinite element of K counts as NaN.  Over FP8 and F16 pages f32 queries enter the
- * products as two f16 terms: |q| (prefill) and |q| * scale * 1.45 (decode) must stay below 65 504. */
+ * a row it does see enters by the formula, but an infinite element of K counts as NaN and one of V gives an infinity or NaN.
+ * Over FP8 and F16 pages f32 queries enter the products as two f16 terms: |q| (prefill) and |q| * scale * 1.45 (decode)
+ * must stay below 65 504.  Elements of V in F32 pages must stay below 2^110: weights are kept up to 2^14 until the end. */
 typedef struct vfkv_paged_attn_params {
     uint32_t n_heads;
     uint32_t window;   /* 0: all keys up to the query's own */
@@ -604,8 +605,8 @@ typedef struct vfkv_paged_attn_params {
     uint32_t io_dtype; /* VFKV_F32 / VFKV_F16: type of q and o */
     uint32_t q_stride; /* elements between two tokens' rows; 0: n_heads * head_dim */
     uint32_t o_stride;
-    float scale;       /* positive, finite */
-    float softcap;     /* as in vfkv_decode_attention; 0: none */
+    float scale;       /* 1e-30 .. 1e30 */
+    float softcap;     /* as in vfkv_decode_attention; 0: none, else 1e-30 .. 1e30 */
 } vfkv_paged_attn_params;
 
 /* Scratch of the two attention calls for one cache geometry; independent of the number and length of the sequences.  Calls that

@@ -226,3 +226,13 @@ def test_workspace_refusals():
     assert L.vfkv_paged_workspace_create(c.handle, 0, C.byref(h)) == -1
     assert L.vfkv_paged_workspace_create(None, 2, C.byref(h)) == -1
     assert L.vfkv_paged_workspace_create(c.handle, 2, None) == -1
+
+
+@pytest.mark.parametrize("call", ["decode", "prefill"])
+@pytest.mark.parametrize("kw", [dict(scale=1e-38), dict(scale=1e31), dict(softcap=1e-39), dict(softcap=3e38), dict(softcap=float("inf"))])
+def test_scale_and_softcap_that_leave_the_normal_numbers_are_refused(ext, call, kw):
+    # (their reciprocals and products with log2 e would be infinite or zero: 0 * inf is NaN)
+    L = _ffi.lib()
+    fn = L.vfkv_paged_decode_attention if call == "decode" else L.vfkv_paged_prefill_attention
+    assert fn(ext.handle, 0, C.byref(batch()), C.byref(attn(**kw)), FAKE, 2 * FAKE, None, None) == -1
+    assert list(kw)[0].encode() in L.vfkv_last_error()

@@ -461,9 +461,11 @@ static int paged_attention(vfkv_pages* c, uint32_t layer, const vfkv_seq_batch* 
     if (p->n_heads == 0u || p->n_heads % kvh != 0u)
         return fail(VFKV_ERR_INVALID_ARG, "%s: n_heads (%u) is not a multiple of n_kv_heads (%u)", who, p->n_heads, kvh);
     if (p->n_heads > 65536u) return fail(VFKV_ERR_UNSUPPORTED, "%s: %u heads", who, p->n_heads);
-    if (!(p->scale > 0.f) || !std::isfinite(p->scale))
-        return fail(VFKV_ERR_INVALID_ARG, "%s: scale must be positive and finite (got %g)", who, (double)p->scale);
-    if (!(p->softcap >= 0.f) || !std::isfinite(p->softcap)) return fail(VFKV_ERR_INVALID_ARG, "%s: softcap must be >= 0 and finite", who);
+    // (the kernels work with scale * log2 e and with the soft-cap's reciprocal: neither may leave the normal numbers)
+    if (!(p->scale >= 1e-30f && p->scale <= 1e30f))
+        return fail(VFKV_ERR_INVALID_ARG, "%s: scale must be between 1e-30 and 1e30 (got %g)", who, (double)p->scale);
+    if (p->softcap != 0.f && !(p->softcap >= 1e-30f && p->softcap <= 1e30f))
+        return fail(VFKV_ERR_INVALID_ARG, "%s: softcap must be 0 or between 1e-30 and 1e30 (got %g)", who, (double)p->softcap);
     if ((rc = row_stride(p->q_stride, (uint64_t)p->n_heads * hd, who, "q", &L.q_stride)) != VFKV_OK) return rc;
     if ((rc = row_stride(p->o_stride, (uint64_t)p->n_heads * hd, who, "o", &L.o_stride)) != VFKV_OK) return rc;
     if (decode && b->q_offsets) return fail(VFKV_ERR_INVALID_ARG, "%s: one token per sequence (q_offsets must be NULL)", who);

@@ -144,6 +144,7 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
     t1 = __builtin_amdgcn_readfirstlane(t1);
     const uint32_t n_rows = (t1 - t0) * group;               // (n_tokens * n_heads <= 2^30)
     const uint32_t row0 = (bi - __builtin_amdgcn_readfirstlane(pre[s])) * R;
+    if (row0 >= n_rows) return;                              // (offsets that overlap can wrap the sums of the line)
     __syncthreads();                                         // the prefix sums have been read: the buffers are free
     const uint32_t row1 = n_rows - row0 < R ? n_rows : row0 + R;
     const int kv_len = (int)__builtin_amdgcn_readfirstlane(paged_kv_len(a.s, s));
