@@ -478,7 +478,7 @@ int vfkv_prefill_attention_gated(vfkv_cache* c, uint32_t layer, uint32_t kv_laye
 typedef struct vfkv_pages_config {
     uint32_t n_layers;
     uint32_t n_kv_heads;
-    uint32_t head_dim;  /* <= 512; multiples of 16 up to 256 run on the matrix cores */
+    uint32_t head_dim;  /* <= 512; multiples of 16 run on the matrix cores (F32: up to 256) */
     uint32_t page_size; /* positions per page: 16, 32, 64, 128 or 256 */
     uint32_t n_pages;   /* n_pages * page_size <= 2^31 - 1 */
     uint32_t dtype;     /* vfkv_dtype */
@@ -589,7 +589,7 @@ typedef struct vfkv_paged_rows {
 int vfkv_paged_qk_rope_kv_write(vfkv_pages* c, uint32_t layer, const vfkv_seq_batch* b, const vfkv_paged_rows* rows,
                                 const vfkv_mrope_params* p, vfkv_stream stream);
 
-/* Both attention calls run on the matrix cores for head_dim a multiple of 16 up to 256 with q and o 16-byte aligned and strides a
+/* Both attention calls run on the matrix cores for head_dim a multiple of 16 (over F32 pages: up to 256) with q and o 16-byte aligned and strides a
  * multiple of 16 bytes; everything else takes a generic kernel (vfkv_last_note says so).  o must not overlap q.
  *
  * What a query sees and how its scores are formed.  The query at position p sees key j when j <= p and

@@ -764,3 +764,68 @@ def test_generic_kernel_leaves_a_note():
             call(0, pool.batch(), q, torch.empty_like(q))
             assert (text in note()) if text else note() == b""
     torch.cuda.synchronize()
+
+
+@CALL
+@IOS
+@pytest.mark.parametrize("dtype", [F16, F8])
+@pytest.mark.parametrize("d, hq, hkv, page", [(512, 8, 1, 64), (512, 4, 4, 16), (272, 6, 2, 32), (320, 33, 1, 128), (448, 16, 2, 256)])
+def test_rows_wider_than_256(d, hq, hkv, page, dtype, io, decode):
+    from vulkanforge_amd import _ffi
+    kv = [130, 1, 0, 700, 33]
+    q_len = [1] * 5 if decode else [130, 1, 0, 65, 20]
+    check_attention(Pool(dtype, hkv, d, page, kv), hq, q_len, io, decode=decode)
+    assert _ffi.lib().vfkv_last_note() == b""                  # (the matrix-core kernels, not the generic one)
+    check_attention(Pool(dtype, hkv, d, page, kv), hq, q_len, io, window=37, sink=5, softcap=20.0, decode=decode)
+
+
+@IOS
+@pytest.mark.parametrize("dtype", [F16, F8])
+def test_rows_wider_than_256_over_long_contexts(dtype, io):
+    # few rows: the keys go to many workgroups and are joined
+    for d in (512, 336):
+        pool = Pool(dtype, 2, d, 64, [5000, 40])
+        check_attention(pool, 8, [1, 1], io, decode=True)
+        check_attention(pool, 8, [7, 3], io)
+        check_attention(pool, 8, [7, 3], io, window=2000, sink=70)
+
+
+@IOS
+@pytest.mark.parametrize("dtype", [F16, F8])
+def test_wide_rows_hide_what_is_not_seen(dtype, io):
+    """Pages that are not there, and V elements that are not finite, in every quarter of a row of 512 elements."""
+    bad = float("nan") if dtype == F8 else float("inf")
+    pool = Pool(dtype, 1, 512, 16, [100, 50])
+    pool.table[0, 2] = -1
+    pool.table[1, 0] = 10 ** 6
+    pool.table_dev.copy_(pool.table)
+    check_attention(pool, 4, [40, 50], io)
+    check_attention(pool, 4, [1, 1], io, decode=True)
+    for hq, m, window in ((2, 70, 0), (8, 40, 20)):
+        pool, clean = (Pool(dtype, 1, 512, 16, [m + 30]) for _ in range(2))
+        at = m + 10
+        p, sl = int(pool.table[0, at // 16]), at % 16
+        row = pool.v[0, p, 0, sl].float().clone()
+        odd = [5, 200, 300, 511]
+        row[odd] = bad
+        pool.v[0, p, 0, sl] = row.to(pool.v.dtype)
+        q = rand_q(m, hq, 512, io)
+        o = [torch.zeros_like(q) for _ in range(2)]
+        for x, y in zip((pool, clean), o):
+            vf.PagedForward(x.cache, hq).prefill_attention(0, x.batch([m]), q, y, window=window)
+        torch.cuda.synchronize()
+        pos = torch.arange(30, m + 30, device=DEV)
+        sees = (pos >= at) & ((pos - window < at) if window else True)
+        hit = ~o[0].isfinite()
+        want = torch.zeros_like(hit)
+        want[:, :, odd] = sees[:, None, None]
+        assert torch.equal(hit, want)
+        assert torch.equal(o[0][~hit], o[1][~hit])
+
+
+def test_f32_pages_wider_than_256_take_the_generic_kernel():
+    from vulkanforge_amd import _ffi
+    pool = Pool(F32, 1, 512, 16, [70, 3])
+    for decode, q_len in ((True, [1, 1]), (False, [30, 3])):
+        check_attention(pool, 2, q_len, decode=decode)
+        assert b"generic" in _ffi.lib().vfkv_last_note()

@@ -64,7 +64,7 @@ struct PagedCopyLaunch {
 
 hipError_t launch_paged_copy(const PagedCopyLaunch& L, hipStream_t stream);
 hipError_t launch_paged_write(const PagedWriteLaunch& L, hipStream_t stream);
-// Matrix-core kernels: head_dim a multiple of 16 up to 256; q and o 16-byte aligned with strides that keep every row so.
+// Matrix-core kernels: head_dim a multiple of 16 up to 512 (F32 pages: 256); q and o 16-byte aligned with strides that keep every row so.
 hipError_t launch_paged_decode(const PagedAttnLaunch& L, hipStream_t stream);
 hipError_t launch_paged_prefill(const PagedAttnLaunch& L, hipStream_t stream);
 hipError_t launch_paged_prefill_full(const PagedAttnLaunch& L, hipStream_t stream);    // F32 pages

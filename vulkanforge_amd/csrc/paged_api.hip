@@ -492,7 +492,7 @@ static int paged_attention(vfkv_pages* c, uint32_t layer, const vfkv_seq_batch* 
     vfkv::clear_note();
     const uint32_t per16 = p->io_dtype == VFKV_F32 ? 4u : 8u;
     const bool aligned = (((uintptr_t)q | (uintptr_t)o) & 15u) == 0u && L.q_stride % per16 == 0u && L.o_stride % per16 == 0u;
-    if (hd % 16u != 0u || hd > 256u || !aligned) {
+    if (hd % 16u != 0u || hd > (c->cfg.dtype == VFKV_F32 ? 256u : 512u) || !aligned) {
         VFKV_HIP(vfkv::launch_paged_generic(L, S(stream)));
         vfkv::note_generic(who, c->cfg.dtype, hd);
         return VFKV_OK;

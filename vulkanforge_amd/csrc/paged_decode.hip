@@ -21,8 +21,9 @@
 //         in its own registers -- no LDS, no barrier.
 //     F32 caches use the f32 matrix instruction with the same ownership; nothing needs turning there.
 // Measured, one layer (copy rate of the card: 5.2 TB/s): 48 sequences of 17-8 193 keys, FP8, 32 / 8 / 128: 80.6 us = 4.8 TB/s; 12 windows
-// of 4 096 keys, F16, 16 / 8 / 256, soft-capped: 82.4 us = 4.6 TB/s; one sequence of 65 536 keys: 25.8 us for the worker (5.2 TB/s) and
-// 6.0 us for the join; one of 200 keys 6.5 us (the chain length -> page -> rows -> join of the wavefronts).
+// of 4 096 keys, F16, 16 / 8 / 256, soft-capped: 77.1 us = 5.0 TB/s; one sequence of 65 536 keys: 25.8 us for the worker (5.2 TB/s) and
+// 6.0 us for the join; one of 200 keys 6.5 us (the chain length -> page -> rows -> join of the wavefronts).  Rows of 512, 48 sequences of
+// up to 8 000 keys, 8 KV heads: FP8 310 us = 5.1 TB/s, F16 538 us = 5.8 TB/s.
 //
 //   - The running maximum is only raised when a score exceeds it by 2^8: weights are kept times 2^6 (at most 2^14 in f16, smallest
 //     step 2^-30 of the largest), and the accumulators are rescaled a few times per sequence instead of once per unit.
@@ -54,6 +55,10 @@ struct DecShape {
     static constexpr int VP = NT / PE;                   // V pieces
     static constexpr int PW = PE * ES / 4;               // dwords of a V piece
     static constexpr int VW = VP * PW;                   // V dwords per lane and key
+    // Rows of 512: two units in registers beside the sums and queries do not fit (F16: 387 registers spilled).  One, whose K half is
+    // requested again when the scores are there and whose V half when the outputs are.  (FP8, where two fit through copies to the
+    // accumulation registers, 64 sequences of 200-600 keys: two / one 48.2 / 45.3 us.)
+    static constexpr bool ONE = D == 512;
 };
 
 // Units of a sequence of n keys: first tokens, then the window of the query at position n - 1.
@@ -130,7 +135,7 @@ __device__ __forceinline__ void unit_prefix(const PagedAttnLaunch& a, uint32_t* 
 }
 
 template <int DT, int D, int SUB>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_decode_kernel(PagedAttnLaunch a, uint32_t n_wg, uint32_t slices, uint32_t direct) {
+__global__ __launch_bounds__(256, D >= 256 ? 1 : 2) void paged_decode_kernel(PagedAttnLaunch a, uint32_t n_wg, uint32_t slices, uint32_t direct) {
     using Z = DecShape<DT, D, SUB>;
     constexpr int OP = D + 4;                                            // pitch of an output row in LDS
     __shared__ __attribute__((aligned(16))) float o_lds[kDecWaves][kDecHeads][OP];
@@ -268,7 +273,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_decode_kernel(Pag
             }
             return r;
         };
-        auto load = [&](Stage& st, const Pages& P, uint32_t u) {         // past the end: the last unit again, from the cache
+        auto load = [&](Stage& st, const Pages& P, uint32_t u, bool ks = true, bool vs = true) {   // past the end: the last unit again, from the cache
             const uint32_t kb = unit_key(u < ub ? u : ub - 1u);
 #pragma unroll
             for (int t = 0; t < SUB; ++t) {
@@ -279,7 +284,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_decode_kernel(Pag
                 const uint8_t* const kp = a.c.k + off;
                 const uint8_t* const vp = a.c.v + off;
 #pragma unroll
-                for (int x = 0; x < Z::KL; ++x) st.k[t][x] = *reinterpret_cast<const u32x4*>(kp + koff[x]);
+                for (int x = 0; x < Z::KL; ++x)
+                    if (ks) st.k[t][x] = *reinterpret_cast<const u32x4*>(kp + koff[x]);
+                if (!vs) continue;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -299,7 +306,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_decode_kernel(Pag
                     }
             }
         };
-        auto compute = [&](Stage& st, const Pages& P, uint32_t u) {
+        auto compute = [&](Stage& st, const Pages& P, uint32_t u, auto&& scored) {
             const uint32_t kb = unit_key(u);
             bool full = kb + (uint32_t)Z::UK <= Q.n && (kb >= Q.lo || kb + (uint32_t)Z::UK <= Q.sink);
 #pragma unroll
@@ -335,6 +342,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_decode_kernel(Pag
                     for (int i = 0; i < 4; ++i) x[t][i] = ror8_sum(sc[i]);
                 }
             }
+            scored();                                                    // (K is used up)
             if (a.softcap > 0.f) {
 #pragma unroll
                 for (int t = 0; t < SUB; ++t)
@@ -431,23 +439,39 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_decode_kernel(Pag
         };
 
         if (ua + (uint32_t)w < ub) {
-            Stage st0, st1;
-            uint32_t u = ua + (uint32_t)w;
-            Pages p0 = get_pages(u), p1 = get_pages(u + kDecWaves);
-            load(st0, p0, u);
-            for (;;) {
-                Pages p2 = get_pages(u + 2u * kDecWaves);
-                load(st1, p1, u + kDecWaves);
-                compute(st0, p0, u);
-                u += kDecWaves;
-                if (u >= ub) break;
-                p0 = p2;
-                p2 = get_pages(u + 2u * kDecWaves);
-                load(st0, p0, u + kDecWaves);
-                compute(st1, p1, u);
-                u += kDecWaves;
-                if (u >= ub) break;
-                p1 = p2;
+            if constexpr (Z::ONE) {
+                Stage st;
+                uint32_t u = ua + (uint32_t)w;
+                Pages p0 = get_pages(u), p1 = get_pages(u + kDecWaves);
+                load(st, p0, u);
+                for (;;) {
+                    const Pages p2 = get_pages(u + 2u * kDecWaves);
+                    compute(st, p0, u, [&] { load(st, p1, u + kDecWaves, true, false); });
+                    load(st, p1, u + kDecWaves, false, true);
+                    u += kDecWaves;
+                    if (u >= ub) break;
+                    p0 = p1;
+                    p1 = p2;
+                }
+            } else {
+                Stage st0, st1;
+                uint32_t u = ua + (uint32_t)w;
+                Pages p0 = get_pages(u), p1 = get_pages(u + kDecWaves);
+                load(st0, p0, u);
+                for (;;) {
+                    Pages p2 = get_pages(u + 2u * kDecWaves);
+                    load(st1, p1, u + kDecWaves);
+                    compute(st0, p0, u, [] {});
+                    u += kDecWaves;
+                    if (u >= ub) break;
+                    p0 = p2;
+                    p2 = get_pages(u + 2u * kDecWaves);
+                    load(st0, p0, u + kDecWaves);
+                    compute(st1, p1, u, [] {});
+                    u += kDecWaves;
+                    if (u >= ub) break;
+                    p1 = p2;
+                }
             }
         }
 
@@ -636,11 +660,17 @@ hipError_t launch_dec(const PagedAttnLaunch& L, hipStream_t stream) {
     // A workgroup per sequence, without the prefix sums and without a join: up to eight units per wavefront, up to sixteen when there
     // are two workgroups per CU or more.  (FP8 heads of 128, 8 KV heads, dealt / a workgroup each: 64 sequences of 200-600 keys
     // 25.5 / 15.8 us, one of 1 000 12.8 / 11.8, 64 of 1 000-2 000 51.1 / 45.1, 16 of 1 000-4 000 25.4 / 32.1.)
-    if (per_seq <= 8u * kDecWaves || (per_seq <= 16u * kDecWaves && (uint64_t)L.s.n_seqs * n_hg >= 512u)) {
+    // (Rows of 512: a quarter of the wavefronts are resident and a unit is a longer way, so half of that, and from half a workgroup per
+    // CU on.  64 FP8 sequences of 200-600 keys, 2 KV heads: 40.9 / 30.2 us; one of 1 000 22.5 / 37.3.)
+    constexpr uint32_t SHORT = D == 512 ? 4u : 8u, FULL = D == 512 ? 128u : 512u;
+    if (per_seq <= SHORT * kDecWaves || (per_seq <= 16u * kDecWaves && (uint64_t)L.s.n_seqs * n_hg >= FULL)) {
         hipLaunchKernelGGL((paged_decode_kernel<DT, D, SUB>), dim3(n_hg, L.s.n_seqs), dim3(256), 0, stream, L, L.s.n_seqs, slices, 1u);
         return hipGetLastError();
     }
+    // as many workgroups as are resident: two per CU, one from rows of 256 on (FP8 rows of 256, 2 KV heads, 48 sequences of up to
+    // 8 000 keys, two / one: 62.7 / 53.9 us; F32, 64 of 200-600: 54.5 / 40.3)
     uint64_t n = paged_decode_wgs(n_hg);
+    if (D >= 256) n = (n + 1u) / 2u;
     const uint64_t useful = (L.s.n_seqs * (per_seq + kBegin) + kBegin + 2u * kDecWaves - 1u) / (kBegin + 2u * kDecWaves);
     if (n > useful) n = useful;
     const uint64_t fits = L.scratch_rows / (2u * (uint64_t)L.n_heads);
@@ -660,12 +690,14 @@ hipError_t launch_paged_decode(const PagedAttnLaunch& L, hipStream_t stream) {
     if (L.c.dtype == kF8) {
         if (d <= 64u) return launch_dec<kF8, 64, 4>(L, stream);
         if (d <= 128u) return launch_dec<kF8, 128, 2>(L, stream);
-        return launch_dec<kF8, 256, 2>(L, stream);
+        if (d <= 256u) return launch_dec<kF8, 256, 2>(L, stream);
+        return launch_dec<kF8, 512, 1>(L, stream);
     }
     if (L.c.dtype == kF16) {
         if (d <= 64u) return launch_dec<kF16, 64, 2>(L, stream);
         if (d <= 128u) return launch_dec<kF16, 128, 2>(L, stream);
-        return launch_dec<kF16, 256, 1>(L, stream);
+        if (d <= 256u) return launch_dec<kF16, 256, 1>(L, stream);
+        return launch_dec<kF16, 512, 1>(L, stream);
     }
     if (d <= 64u) return launch_dec<kF32, 64, 1>(L, stream);
     if (d <= 128u) return launch_dec<kF32, 128, 1>(L, stream);

@@ -102,14 +102,16 @@ __device__ __forceinline__ void block_prefix(const PagedAttnLaunch& a, uint32_t 
     __syncthreads();
 }
 
-template <int DT, int D, bool IOF16, bool CAP, int KT, int CK, int NW, int MINW>
+template <int DT, int D, bool IOF16, bool CAP, int KT, int CK, int NW, int MINW, int DS = 1>
 __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnLaunch a, uint32_t n_split) {
     using Z = PreShape<DT, D, KT, NW>;
     constexpr bool F32C = DT == kF32;
     constexpr bool PAIR = !IOF16 && !F32C;                   // queries and weights as value + remainder
     constexpr int NB = CK / 32;                              // 32-key blocks per chunk: what a wavefront takes through both products at once
-    constexpr int DT32 = D / 32;
-    constexpr uint32_t R = 32u * NW;
+    constexpr int DW = D / DS;                               // columns of a wavefront: DS wavefronts share 32 rows
+    constexpr int DT32 = DW / 32;
+    constexpr uint32_t R = 32u * NW / DS;
+    static_assert(DS == 1 || (DS == 2 && KT == CK && !F32C), "the shared scores are joined once per tile");
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];   // two buffers; before the first tile, the prefix sums
     __shared__ uint32_t wave_sum[NW];
     // keys whose V row holds an infinity or NaN, from tiles that are hidden in part: at most the tiles the block's queries and
@@ -162,7 +164,7 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
     auto tile_key = [&](uint32_t t) { return (t < sink_tiles ? t : first + t - sink_tiles) * (uint32_t)KT; };
 
     // ---- this wavefront's rows
-    const uint32_t wr0 = row0 + (uint32_t)w * 32u;
+    const uint32_t wr0 = row0 + (uint32_t)(w / DS) * 32u, dw0 = (uint32_t)(w % DS) * DW;   // first row, first column
     const bool wave_has = wr0 < row1;
     const uint32_t wr1 = row1 < wr0 + 32u ? row1 : wr0 + 32u;
     const int wmin = wave_has ? pos0 + (int)(wr0 / group) : 0, wmax = wave_has ? pos0 + (int)((wr1 - 1u) / group) : -1;
@@ -184,7 +186,7 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
         tok += t0;
     }
     // ---- Q^T operands
-    half8_t qh[F32C ? 1 : D / 16], ql[PAIR ? D / 16 : 1];
+    half8_t qh[F32C ? 1 : DW / 16], ql[PAIR ? DW / 16 : 1];
     float qf[F32C ? D / 2 : 1];
     {
         const uint64_t at = (uint64_t)tok * a.q_stride + (uint64_t)head * dr;
@@ -206,8 +208,8 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
             }
         } else {
 #pragma unroll
-            for (int c = 0; c < D / 16; ++c) {
-                const uint32_t d = 16u * c + 8u * (uint32_t)hf;
+            for (int c = 0; c < DW / 16; ++c) {
+                const uint32_t d = dw0 + 16u * c + 8u * (uint32_t)hf;
                 const bool ok = real && d < dr;
                 if constexpr (IOF16) {
                     const half8_t x = *reinterpret_cast<const half8_t*>(reinterpret_cast<const _Float16*>(a.q) + at + (ok ? d : 0u));
@@ -334,10 +336,8 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
     };
 
     // ---- one tile
-    auto compute = [&](bool masked, int buf, const uint32_t (&pages)[CK / 16], int chunk_at, int kb) {   // masked: some of the queries do not see some of the keys
-        const uint8_t* const kl = lds + buf * Z::BUF + chunk_at * Z::KPITCH;
-        const uint8_t* const vl = lds + buf * Z::BUF + KT * Z::KPITCH + chunk_at * Z::VPITCH;
-        float16_t sc[NB];
+    auto scores = [&](float16_t (&sc)[NB], int buf, int chunk_at) {
+        const uint8_t* const kl = lds + buf * Z::BUF + chunk_at * Z::KPITCH + dw0 * Z::LE;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
 #pragma unroll
@@ -352,13 +352,16 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
                 }
             } else {
 #pragma unroll
-                for (int c = 0; c < D / 16; ++c) {
+                for (int c = 0; c < DW / 16; ++c) {
                     const half8_t k = *reinterpret_cast<const half8_t*>(krow + 32 * c);
                     sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[c], sc[b], 0, 0, 0);
                     if constexpr (PAIR) sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[c], sc[b], 0, 0, 0);
                 }
             }
         }
+    };
+    auto finish = [&](float16_t (&sc)[NB], bool masked, int buf, const uint32_t (&pages)[CK / 16], int chunk_at, int kb) {   // masked: some of the queries do not see some of the keys
+        const uint8_t* const vl = lds + buf * Z::BUF + KT * Z::KPITCH + chunk_at * Z::VPITCH + dw0 * Z::LE;
         if constexpr (CAP) {
 #pragma unroll
             for (int b = 0; b < NB; ++b)
@@ -460,7 +463,7 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
             __syncthreads();                                   // tile t staged by all; tile t - 1 no longer read
             const Pages p2 = get_pages(t + 2u);
             if (t + 1u < tb) fetch(p1, t + 1u);
-            if (wave_has) {
+            if (wave_has || DS > 1) {
                 auto one = [&](int c) {
                     const int kb = (int)tile_key(t) + c;
                     uint32_t pages[CK / 16];
@@ -473,8 +476,35 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
                         ghost = ghost || pages[i] >= a.c.n_pages;
                     }
                     // (a chunk that none of the wavefront's queries sees is passed over)
-                    if (!(kb > wmax || ((uint32_t)kb >= a.n_sink && kb + CK <= wlo_min)))
-                        compute(!(kb + CK - 1 <= wmin && (kb >= wlo_max || (uint32_t)(kb + CK) <= a.n_sink) && !ghost), buf, pages, c, kb);
+                    const bool none = kb > wmax || ((uint32_t)kb >= a.n_sink && kb + CK <= wlo_min);
+                    auto masked = [&] { return !(kb + CK - 1 <= wmin && (kb >= wlo_max || (uint32_t)(kb + CK) <= a.n_sink) && !ghost); };
+                    if constexpr (DS == 1) {
+                        if (none) return;
+                        float16_t sc[NB];
+                        scores(sc, buf, c);
+                        finish(sc, masked(), buf, pages, c, kb);
+                    } else {                                    // sums over half of the columns each: added, in either order the same
+                        float4_t* const mine = reinterpret_cast<float4_t*>(lds + 2 * Z::BUF) + w * (NB * 256) + lane;
+                        const float4_t* const other = reinterpret_cast<const float4_t*>(lds + 2 * Z::BUF) + (w ^ 1) * (NB * 256) + lane;
+                        float16_t sc[NB];
+                        const bool any = wave_has && !none;
+                        if (any) {
+                            scores(sc, buf, c);
+#pragma unroll
+                            for (int x = 0; x < 4 * NB; ++x)
+                                mine[64 * x] = float4_t{sc[x / 4][4 * (x % 4)], sc[x / 4][4 * (x % 4) + 1], sc[x / 4][4 * (x % 4) + 2], sc[x / 4][4 * (x % 4) + 3]};
+                        }
+                        __syncthreads();
+                        if (any) {
+#pragma unroll
+                            for (int x = 0; x < 4 * NB; ++x) {
+                                const float4_t y = other[64 * x];
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) sc[x / 4][4 * (x % 4) + j] += y[j];
+                            }
+                            finish(sc, masked(), buf, pages, c, kb);
+                        }
+                    }
                 };
                 if constexpr (KT == CK) one(0);
                 else
@@ -493,12 +523,12 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
     const uint64_t at = (uint64_t)tok * a.o_stride + (uint64_t)head * dr;
     if (real) {
         const float inv = n_split > 1u ? 1.0f : L != 0.f ? 1.0f / L : 0.f;
-        if (n_split > 1u && hf == 0) { a.scratch_max[row] = m; a.scratch_sum[row] = L; }
+        if (n_split > 1u && hf == 0 && dw0 == 0u) { a.scratch_max[row] = m; a.scratch_sum[row] = L; }
 #pragma unroll
         for (int n = 0; n < DT32; ++n)
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
-                const uint32_t d = 32u * n + 8u * b + 4u * (uint32_t)hf;
+                const uint32_t d = dw0 + 32u * n + 8u * b + 4u * (uint32_t)hf;
                 if (d >= dr) continue;
                 float4_t v;
 #pragma unroll
@@ -526,7 +556,7 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
         const uint8_t* const vrow = a.c.v + (uint64_t)(page < a.c.n_pages ? page : 0u) * a.c.page_bytes + (head_rows + (key & slot_mask)) * row_b;
         if (!real || !(key - lo < span || key < lead)) continue;
 #pragma unroll 1
-        for (uint32_t d = 4u * (uint32_t)hf; d < dr; d += 8u)
+        for (uint32_t d = dw0 + 4u * (uint32_t)hf; d < dr && d < dw0 + DW; d += 8u)
 #pragma unroll 1
             for (uint32_t j = d; j < d + 4u; ++j) {
                 const float v = load_kv_elem(vrow, DT, j);
@@ -546,10 +576,11 @@ bool blocks_alike(const PagedAttnLaunch& L) {
     return L.max_kv >= 2u * chunk || (L.window != 0u && chunk >= 2u * (uint64_t)L.window);
 }
 
-template <int DT, int D, bool IOF16, bool CAP, int KT, int CK, int NW, int MINW>
+template <int DT, int D, bool IOF16, bool CAP, int KT, int CK, int NW, int MINW, int DS = 1>
 hipError_t launch_pre(const PagedAttnLaunch& L, hipStream_t stream) {
     using Z = PreShape<DT, D, KT, NW>;
-    constexpr uint64_t R = 32u * NW;
+    constexpr uint64_t R = 32u * NW / DS;
+    constexpr uint32_t LDS = 2u * Z::BUF + (DS > 1 ? NW * 64u * CK * 2u : 0u);   // (DS > 1: the scores in f32)
     const uint64_t group = L.n_heads / L.c.n_kv_heads;
     // a sequence's last block may be ragged: at most one block more per sequence that has rows
     const uint64_t with_rows = L.s.n_seqs < L.s.n_tokens ? L.s.n_seqs : L.s.n_tokens;
@@ -560,7 +591,7 @@ hipError_t launch_pre(const PagedAttnLaunch& L, hipStream_t stream) {
     // reads the parts once (about 4 TB/s and 3 us).  A tile takes about 2.2 us for f16 rows of 128 elements, 1.6 times that with
     // value + remainder, 6.8 us for 32 keys on the f32 instruction.  (FP8, 32 / 8 / 128, one part against two: 1 024 f16 tokens from
     // position 0 33.6 / 39.5 us, over 5 000 keys 162 / 104 us; 7 tokens over 1 000 keys, F16 heads of 64, 4 / 16 parts 17.6 / 12.6 us.)
-    constexpr uint64_t tile_ns = (DT == kF32 ? 6800u * KT / 32u : (IOF16 ? 2200u : 3500u) * KT / 64u) * D / 128u;
+    constexpr uint64_t tile_ns = (DT == kF32 ? 6800u * KT / 32u : (IOF16 ? 2200u : 3500u) * KT / 64u) * (D / DS) / 128u;
     const uint64_t likely = (L.s.n_tokens * group + R - 1u) / R * L.c.n_kv_heads;
     // (unlike blocks: twice the workgroups that fit, so that the last ones are short; F16 rows of 256, 2 048 tokens 129 -> 105 us)
     const uint64_t room = 256u * MINW * 4u / NW * (blocks_alike(L) ? 1u : 2u);
@@ -576,8 +607,8 @@ hipError_t launch_pre(const PagedAttnLaunch& L, hipStream_t stream) {
         const uint64_t ns = (tiles + i - 1u) / i * tile_ns + 3000u + rows * i * L.c.head_dim * 8u / 4000u;
         if (ns < best) { best = ns; n = i; }
     }
-    hipLaunchKernelGGL((paged_prefill_kernel<DT, D, IOF16, CAP, KT, CK, NW, MINW>), dim3((uint32_t)(blocks * L.c.n_kv_heads), (uint32_t)n), dim3(NW * 64),
-                       2u * Z::BUF, stream, L, (uint32_t)n);
+    hipLaunchKernelGGL((paged_prefill_kernel<DT, D, IOF16, CAP, KT, CK, NW, MINW, DS>), dim3((uint32_t)(blocks * L.c.n_kv_heads), (uint32_t)n), dim3(NW * 64),
+                       LDS, stream, L, (uint32_t)n);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || n == 1u) return e;
     return launch_paged_rows_merge(L, (uint32_t)n, stream);
@@ -601,6 +632,10 @@ hipError_t launch_dim(const PagedAttnLaunch& L, hipStream_t stream) {
         constexpr int CK = IOF16 ? 64 : 32, KT = 64;
         if (d <= 64u) return many ? launch_pre<DT, 64, IOF16, CAP, 64, 64, 8, 2>(L, stream) : launch_pre<DT, 64, IOF16, CAP, 64, 64, 4, 2>(L, stream);
         if (d <= 128u) return many ? launch_pre<DT, 128, IOF16, CAP, KT, CK, 8, 2>(L, stream) : launch_pre<DT, 128, IOF16, CAP, KT, CK, 4, 2>(L, stream);
+        // rows of 512: two wavefronts per block of 32 rows, each half of the columns of both products, their scores added through LDS
+        // (16 / 2 heads, FP8, f16 rows: 512 tokens over 4 096 keys 215 us = 340 TFLOP/s, 4 096 from position 0 688 us = 400; one
+        // workgroup per CU, two barriers per tile; the generic kernel: 43 ms)
+        if (d > 256u) return launch_pre<DT, 512, IOF16, CAP, 32, 32, 4, 1, 2>(L, stream);
         if constexpr (IOF16)                                     // (value + remainder of 256 elements do not fit 256 registers)
             if (many) return launch_pre<DT, 256, IOF16, CAP, 32, 32, 8, 2>(L, stream);
         return launch_pre<DT, 256, IOF16, CAP, 32, 32, 4, 1>(L, stream);
