@@ -39,6 +39,20 @@ int main() {
         REQUIRE(prefix_reuse_start({10, 11, 12, 13, 14}, {10, 11, 12, 99}) == 3);
         REQUIRE(prefix_reuse_start({1, 2, 3, 4}, {1, 2, 3, 4}) == 3 && prefix_reuse_start({}, {1, 2, 3}) == 0);
     }
+    {   // page counting of the paged cache: shared full pages, a page of its own for a last one that is not full
+        PagedKvCache c(vfkv_pages_config{2, 2, 64, 16, 8, VFKV_F16}, true);
+        const std::vector<uint32_t> p = c.alloc(c.pages_for(40));
+        REQUIRE((p == std::vector<uint32_t>{0, 1, 2}) && c.free_count() == 5);
+        const auto forks = c.fork(p, 40, 2);
+        REQUIRE((forks[0] == std::vector<uint32_t>{0, 1, 3}) && (forks[1] == std::vector<uint32_t>{0, 1, 4}));
+        REQUIRE(c.refcount(0) == 3 && c.refcount(2) == 1 && c.free_count() == 3);
+        c.release(p);
+        REQUIRE(c.refcount(0) == 2 && c.refcount(2) == 0 && c.free_count() == 4);
+        REQUIRE((c.compact() == std::vector<uint32_t>{0, 1, VFKV_NO_PAGE, 3, 2, VFKV_NO_PAGE, VFKV_NO_PAGE, VFKV_NO_PAGE}));
+        bool threw = false;
+        try { c.alloc(5); } catch (const Error& e) { threw = e.status == VFKV_ERR_WORKSPACE; }
+        REQUIRE(threw);
+    }
     if (vfkv_device_count() == 0) { std::printf("host selftest: layout checks passed (no GPU: compute checks skipped)\n"); return 0; }
 
     const uint32_t H = 32, Hkv = 8, D = 128, ctx = 1000;
@@ -118,6 +132,50 @@ int main() {
         std::printf("fused decode block: max |q_rot - closed form| = %.3g, max |O - V[123]| = %.3g\n", wq, worst);
         REQUIRE(wq < 2e-4 && worst < 1e-6);
         hipFree(dqo); hipFree(dz);
+    }
+    // Paged cache, two sequences: K = 0 makes every weight equal, so O = mean of the rows of V each query sees.
+    {
+        const uint32_t ps = 16, n0 = 40, n1 = 3;
+        PagedForward paged(PagedKvCache(vfkv_pages_config{1, Hkv, D, ps, 8, VFKV_F16}), H);
+        const std::vector<uint32_t> a = paged.cache.alloc(3), b = paged.cache.alloc(1);
+        const int32_t host[] = {(int32_t)a[0], (int32_t)a[1], (int32_t)a[2], (int32_t)b[0], -1, -1, (int32_t)n0, (int32_t)n1, 0, (int32_t)n0, (int32_t)(n0 + n1)};
+        int32_t* dev; float *dz, *dq2, *do2;
+        const size_t n = n0 + n1;
+        hipMalloc(&dev, sizeof host); hipMalloc(&dz, n * row * 4); hipMalloc(&dq2, n * H * D * 4); hipMalloc(&do2, n * H * D * 4);
+        hipMemcpy(dev, host, sizeof host, hipMemcpyHostToDevice);
+        hipMemset(dz, 0, n * row * 4);
+        std::vector<float> q2(n * H * D, 1.0f), o2(q2.size());
+        hipMemcpy(dq2, q2.data(), q2.size() * 4, hipMemcpyHostToDevice);
+        const vfkv_seq_batch batch{dev, dev + 6, dev + 8, 2, 3, (uint32_t)n, 0};
+        vfkv_paged_rows rows{};
+        rows.k = dz; rows.v = dv; rows.io_dtype = VFKV_F32;
+        vfkv_mrope_params none{};
+        none.rope_mode = VFKV_ROPE_NEOX; none.n_axes = 1; none.eps = 1e-6f;
+        paged.qk_rope_kv_write(0, batch, rows, none);
+        paged.prefill_attention(0, batch, paged.params(VFKV_F32), dq2, do2);
+        hipDeviceSynchronize();
+        hipMemcpy(o2.data(), do2, o2.size() * 4, hipMemcpyDeviceToHost);
+        worst = 0;
+        for (uint32_t h = 0; h < H; ++h) for (uint32_t d = 0; d < D; ++d) {
+            double mean = 0;
+            for (size_t t = 0; t < n; ++t) {
+                if (t == n0) mean = 0;
+                mean += v[t * row + (h / 4) * D + d];
+                worst = std::fmax(worst, std::fabs(o2[(t * H + h) * D + d] - mean / (t < n0 ? t + 1 : t - n0 + 1)));
+            }
+        }
+        const vfkv_seq_batch last{dev, dev + 6, nullptr, 2, 3, 2, 0};
+        paged.decode_attention(0, last, paged.params(VFKV_F32), dq2, do2);
+        hipDeviceSynchronize();
+        std::vector<float> o3(2 * H * D);
+        hipMemcpy(o3.data(), do2, o3.size() * 4, hipMemcpyDeviceToHost);
+        for (size_t x = 0; x < H * D; ++x) {
+            worst = std::fmax(worst, std::fabs(o3[x] - o2[(n0 - 1) * H * D + x]));
+            worst = std::fmax(worst, std::fabs(o3[H * D + x] - o2[(n - 1) * H * D + x]));
+        }
+        std::printf("paged cache: max |O - mean(V)| = %.3g\n", worst);
+        REQUIRE(worst < 1e-5);
+        hipFree(dev); hipFree(dz); hipFree(dq2); hipFree(do2);
     }
     bool threw = false;
     try { fwd.step_attention(1, ctx + 1, dq, dout); } catch (const Error& e) { threw = e.status == VFKV_ERR_INVALID_ARG; }

@@ -265,4 +265,88 @@ private:
     vfkv_workspace* ws_ = nullptr;
 };
 
+// ---- paged cache: several sequences over one pool of pages (no counterpart in the reference) ----
+class PagedKvCache {
+public:
+    vfkv_pages_config config;
+
+    // Buffers on the current device; layout_only: page counting without them.
+    explicit PagedKvCache(const vfkv_pages_config& cfg, bool layout_only = false) : config(cfg) {
+        check(layout_only ? vfkv_pages_create_external(&cfg, nullptr, nullptr, &h_) : vfkv_pages_create(&cfg, &h_));
+    }
+    PagedKvCache(PagedKvCache&& o) noexcept : config(o.config), h_(std::exchange(o.h_, nullptr)) {}
+    PagedKvCache(const PagedKvCache&) = delete;
+    PagedKvCache& operator=(const PagedKvCache&) = delete;
+    ~PagedKvCache() { vfkv_pages_destroy(h_); }
+
+    vfkv_pages* handle() const { return h_; }
+    uint32_t pages_for(uint32_t kv_len) const { return (uint32_t)(((uint64_t)kv_len + config.page_size - 1) / config.page_size); }
+    uint32_t free_count() const { return vfkv_pages_free_count(h_); }
+    uint32_t refcount(uint32_t page) const { return vfkv_pages_refcount(h_, page); }
+    std::vector<uint32_t> alloc(uint32_t n) {
+        std::vector<uint32_t> out(n);
+        check(vfkv_pages_alloc(h_, n, out.data()));
+        return out;
+    }
+    void retain(const std::vector<uint32_t>& pages) { check(vfkv_pages_retain(h_, pages.data(), (uint32_t)pages.size())); }
+    void release(const std::vector<uint32_t>& pages) { check(vfkv_pages_release(h_, pages.data(), (uint32_t)pages.size())); }
+    void copy_pages(const std::vector<uint32_t>& src, const std::vector<uint32_t>& dst, const std::vector<uint32_t>* rows = nullptr,
+                    vfkv_stream stream = nullptr) {
+        if (src.size() != dst.size() || (rows && rows->size() != src.size()))
+            throw Error(VFKV_ERR_INVALID_ARG, "copy_pages: src, dst and rows must have the same length");
+        check(vfkv_pages_copy(h_, src.data(), dst.data(), rows ? rows->data() : nullptr, (uint32_t)src.size(), stream));
+    }
+    // One page list per continuation of the kv_len positions in `pages`.
+    std::vector<std::vector<uint32_t>> fork(const std::vector<uint32_t>& pages, uint32_t kv_len, uint32_t n_forks, vfkv_stream stream = nullptr) {
+        const uint32_t used = pages_for(kv_len);
+        if (pages.size() < used) throw Error(VFKV_ERR_INVALID_ARG, "fork: the page list is shorter than kv_len");
+        std::vector<uint32_t> flat((size_t)n_forks * used);
+        check(vfkv_pages_fork(h_, pages.data(), kv_len, n_forks, flat.data(), stream));
+        std::vector<std::vector<uint32_t>> out;
+        for (uint32_t f = 0; f < n_forks; ++f) out.emplace_back(flat.begin() + (size_t)f * used, flat.begin() + (size_t)(f + 1) * used);
+        return out;
+    }
+    // Every page's new id (VFKV_NO_PAGE: the page was free).
+    std::vector<uint32_t> compact(vfkv_stream stream = nullptr) {
+        std::vector<uint32_t> out(config.n_pages);
+        check(vfkv_pages_compact(h_, out.data(), stream));
+        return out;
+    }
+
+private:
+    vfkv_pages* h_ = nullptr;
+};
+
+class PagedForward {
+public:
+    PagedKvCache cache;
+    uint32_t n_heads;
+    float attn_scale;
+    vfkv_stream stream = nullptr;
+
+    PagedForward(PagedKvCache c, uint32_t heads) : cache(std::move(c)), n_heads(heads) {
+        check(vfkv_paged_workspace_create(cache.handle(), n_heads, &ws_));
+        attn_scale = 1.0f / std::sqrt((float)cache.config.head_dim);
+    }
+    PagedForward(const PagedForward&) = delete;
+    PagedForward& operator=(const PagedForward&) = delete;
+    ~PagedForward() { if (ws_) vfkv_workspace_destroy(ws_); }
+
+    void qk_rope_kv_write(uint32_t layer, const vfkv_seq_batch& batch, const vfkv_paged_rows& rows, const vfkv_mrope_params& rope) {
+        check(vfkv_paged_qk_rope_kv_write(cache.handle(), layer, &batch, &rows, &rope, stream));
+    }
+    vfkv_paged_attn_params params(uint32_t io_dtype, uint32_t window = 0, uint32_t n_sink = 0, float softcap = 0.f) const {
+        return vfkv_paged_attn_params{n_heads, window, n_sink, io_dtype, 0, 0, attn_scale, softcap};
+    }
+    void decode_attention(uint32_t layer, const vfkv_seq_batch& batch, const vfkv_paged_attn_params& p, const void* q, void* o) {
+        check(vfkv_paged_decode_attention(cache.handle(), layer, &batch, &p, q, o, ws_, stream));
+    }
+    void prefill_attention(uint32_t layer, const vfkv_seq_batch& batch, const vfkv_paged_attn_params& p, const void* q, void* o) {
+        check(vfkv_paged_prefill_attention(cache.handle(), layer, &batch, &p, q, o, ws_, stream));
+    }
+
+private:
+    vfkv_workspace* ws_ = nullptr;
+};
+
 }  // namespace vfkv
