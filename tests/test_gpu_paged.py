@@ -829,3 +829,25 @@ def test_f32_pages_wider_than_256_take_the_generic_kernel():
     for decode, q_len in ((True, [1, 1]), (False, [30, 3])):
         check_attention(pool, 2, q_len, decode=decode)
         assert b"generic" in _ffi.lib().vfkv_last_note()
+
+
+@CALL
+@DTYPES
+@pytest.mark.parametrize("d", [64, 80, 128, 256, 512])
+def test_tiny_and_huge_queries_keep_their_accuracy(d, dtype, decode):
+    """Queries of any size, with a scale that brings the scores to ordinary sizes: an element counts to 2^-22 of its row's largest."""
+    pool = Pool(dtype, 2, d, 32, [70, 3, 129])
+    q_len = [1] * 3 if decode else [40, 3, 5]
+    for size, softcap in ((2.0 ** -24, 0.0), (2.0 ** -24, 3.0), (2.0 ** 40, 0.0), (2.0 ** -70, 0.0)):
+        q = rand_q(sum(q_len), 4, d, scale=size)
+        q[:, 1] *= 2.0 ** -10                                 # heads of one token far apart
+        scale = 1.0 / (size * math.sqrt(d))
+        o = torch.full_like(q, float("nan"))
+        fwd = vf.PagedForward(pool.cache, 4)
+        call = fwd.decode_attention if decode else fwd.prefill_attention
+        call(0, pool.batch(None if decode else q_len), q, o, scale=scale, softcap=softcap)
+        torch.cuda.synchronize()
+        ref, tol = attention(pool, q, q_len, softcap=softcap, scale=scale)
+        err = (o.cpu().double() - ref).abs().max().item()
+        print(f"{size:.3g} {softcap}: {err:.3g} of {tol:.3g}", flush=True)
+        assert err <= tol

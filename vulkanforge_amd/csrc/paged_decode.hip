@@ -14,7 +14,7 @@
 //     registers one unit ahead.
 //   - Both products run on the matrix cores, transposed, so that no register changes lanes in between:
 //       S^T[key, col] = K Q^T: A = K rows as loaded (FP8 widened exactly), B = Q^T.  Columns 0-7 hold f16(q'), columns 8-15
-//         f16(q' - f16(q')) of the same heads (q' = q * scale * log2 e): the sum of both columns has f32-level accuracy.
+//         f16(q' - f16(q')) of the same heads (q' = q times a power of two): the sum of both columns has f32-level accuracy.
 //       O^T[d, col] += V^T P^T: B = P as the score tile left it (a lane holds four consecutive keys of one column, which is what
 //         the operand wants when the contraction runs over the keys in that order), columns 0-7 f16(p), 8-15 the remainder.
 //         A = V^T: a lane loads D / 16 columns of its four keys per tile and turns that small matrix with byte permutes
@@ -221,10 +221,11 @@ __global__ __launch_bounds__(256, D >= 256 ? 1 : 2) void paged_decode_kernel(Pag
         // ---- q' as the B operand of the first product
         half8_t qb[DT == kF32 ? 1 : D / 32];
         float qf[DT == kF32 ? D / 4 : 1];
+        float fac = 1.0f;                                                 // of the scores, to log2 units
         {
             const bool there = (uint32_t)col < heads && (DT != kF32 || !is_lo);
             const uint64_t qrow = (uint64_t)s * a.q_stride + (uint64_t)(h0 + (there ? (uint32_t)col : 0u)) * dr;
-            auto load8 = [&](uint32_t d, float* out, int n) {             // n = 4 or 8 elements of the head's row, times scale
+            auto load8 = [&](uint32_t d, float* out, int n, float by) {   // n = 4 or 8 elements of the head's row, times `by`
                 const bool ok = there && d < dr;
                 const uint64_t at = qrow + (ok ? d : 0u);
                 for (int j = 0; j < n; j += 4) {
@@ -236,24 +237,33 @@ __global__ __launch_bounds__(256, D >= 256 ? 1 : 2) void paged_decode_kernel(Pag
                         const float4_t f = *reinterpret_cast<const float4_t*>(reinterpret_cast<const float*>(a.q) + at + j);
                         for (int i = 0; i < 4; ++i) x[i] = f[i];
                     }
-                    for (int i = 0; i < 4; ++i) out[j + i] = ok ? x[i] * scale_l2 : 0.f;
+                    for (int i = 0; i < 4; ++i) out[j + i] = ok ? x[i] * by : 0.f;
                 }
             };
             if constexpr (DT == kF32) {
 #pragma unroll
-                for (int x = 0; x < Z::KL; ++x) load8((uint32_t)(4 * x + g) * 4u, &qf[4 * x], 4);
+                for (int x = 0; x < Z::KL; ++x) load8((uint32_t)(4 * x + g) * 4u, &qf[4 * x], 4, scale_l2);
             } else {
+                // times the power of two that brings the row's largest element to [0.5, 1): value + remainder hold every element to
+                // 2^-23 of that, whatever the row's size
+                float x[D / 32][8], top = 0.f;
 #pragma unroll
                 for (int c = 0; c < D / 32; ++c) {
                     constexpr int PER = Z::KE / 8;                       // operands per piece
-                    float x[8];
-                    load8((uint32_t)(4 * (c / PER) + g) * Z::KE + 8u * (uint32_t)(c % PER), x, 8);
+                    load8((uint32_t)(4 * (c / PER) + g) * Z::KE + 8u * (uint32_t)(c % PER), x[c], 8, 1.0f);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[c][j]));
+                }
+                const int e = __builtin_amdgcn_frexp_expf(max_over_groups(top));
+                fac = fmaxf(__builtin_ldexpf(scale_l2, e), 1e-37f);       // (not 0: -inf * 0 of a hidden key would be NaN)
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c)
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const _Float16 hi = (_Float16)x[j];
-                        qb[c][j] = is_lo ? (_Float16)(x[j] - (float)hi) : hi;
+                        const float y = __builtin_ldexpf(x[c][j], -e);
+                        const _Float16 hi = (_Float16)y;
+                        qb[c][j] = is_lo ? (_Float16)(y - (float)hi) : hi;
                     }
-                }
             }
         }
 
@@ -343,11 +353,13 @@ __global__ __launch_bounds__(256, D >= 256 ? 1 : 2) void paged_decode_kernel(Pag
                 }
             }
             scored();                                                    // (K is used up)
+            float to_l2 = fac;
             if (a.softcap > 0.f) {
+                to_l2 = 1.0f;                                            // (the soft-cap leaves log2 units)
 #pragma unroll
                 for (int t = 0; t < SUB; ++t)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) x[t][i] = paged_softcap_l2(x[t][i], cap_l2, inv_cap_l2);
+                    for (int i = 0; i < 4; ++i) x[t][i] = paged_softcap_l2(x[t][i] * fac, cap_l2, inv_cap_l2);
             }
             if (!full) {
 #pragma unroll
@@ -366,8 +378,8 @@ __global__ __launch_bounds__(256, D >= 256 ? 1 : 2) void paged_decode_kernel(Pag
             for (int t = 0; t < SUB; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) mx = fmaxf(mx, x[t][i]);
-            if (__any(mx > m + (kRaise + kBias))) {
-                const float mn = fmaxf(m, max_over_groups(mx) - kBias);
+            if (__any(mx * to_l2 > m + (kRaise + kBias))) {
+                const float mn = fmaxf(m, max_over_groups(mx) * to_l2 - kBias);
                 const float corr = __builtin_amdgcn_exp2f(m - mn);
                 m = mn;
                 l *= corr;
@@ -380,7 +392,7 @@ __global__ __launch_bounds__(256, D >= 256 ? 1 : 2) void paged_decode_kernel(Pag
             for (int t = 0; t < SUB; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    x[t][i] = __builtin_amdgcn_exp2f(x[t][i] - m);
+                    x[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[t][i], to_l2, -m));
                     l += x[t][i];
                 }
             if constexpr (DT == kF32) {

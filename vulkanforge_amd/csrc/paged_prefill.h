@@ -188,6 +188,8 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
     // ---- Q^T operands
     half8_t qh[F32C ? 1 : DW / 16], ql[PAIR ? DW / 16 : 1];
     float qf[F32C ? D / 2 : 1];
+    const float scale_l2 = a.scale * 1.44269504088896f;
+    float qmul = scale_l2;                                   // of the scores, to log2 units
     {
         const uint64_t at = (uint64_t)tok * a.q_stride + (uint64_t)head * dr;
         if constexpr (F32C) {
@@ -206,27 +208,49 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
 #pragma unroll
                 for (int j = 0; j < 4; ++j) qf[4 * c + j] = ok ? x[j] : 0.f;
             }
-        } else {
+        } else if constexpr (IOF16) {
 #pragma unroll
             for (int c = 0; c < DW / 16; ++c) {
                 const uint32_t d = dw0 + 16u * c + 8u * (uint32_t)hf;
                 const bool ok = real && d < dr;
-                if constexpr (IOF16) {
-                    const half8_t x = *reinterpret_cast<const half8_t*>(reinterpret_cast<const _Float16*>(a.q) + at + (ok ? d : 0u));
+                const half8_t x = *reinterpret_cast<const half8_t*>(reinterpret_cast<const _Float16*>(a.q) + at + (ok ? d : 0u));
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) qh[c][j] = ok ? x[j] : (_Float16)0.f;
-                } else {
-                    const float* const src = reinterpret_cast<const float*>(a.q) + at + (ok ? d : 0u);
-                    const float4_t x0 = *reinterpret_cast<const float4_t*>(src), x1 = *reinterpret_cast<const float4_t*>(src + 4);
+                for (int j = 0; j < 8; ++j) qh[c][j] = ok ? x[j] : (_Float16)0.f;
+            }
+        } else {
+            // times the power of two that brings the row's largest element to [0.5, 1): value + remainder hold every element to 2^-23 of
+            // that, whatever the row's size
+            float x[DW / 16][8], top = 0.f;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float x = ok ? (j < 4 ? x0[j & 3] : x1[j & 3]) : 0.f;
-                        const _Float16 hi = (_Float16)x;
-                        qh[c][j] = hi;
-                        ql[c][j] = (_Float16)(x - (float)hi);
-                    }
+            for (int c = 0; c < DW / 16; ++c) {
+                const uint32_t d = dw0 + 16u * c + 8u * (uint32_t)hf;
+                const bool ok = real && d < dr;
+                const float* const src = reinterpret_cast<const float*>(a.q) + at + (ok ? d : 0u);
+                const float4_t x0 = *reinterpret_cast<const float4_t*>(src), x1 = *reinterpret_cast<const float4_t*>(src + 4);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    x[c][j] = ok ? (j < 4 ? x0[j & 3] : x1[j & 3]) : 0.f;
+                    top = fmaxf(top, fabsf(x[c][j]));
                 }
             }
+            top = max_over_halves(top);
+            if constexpr (DS > 1) {                          // the other wavefront's columns of the same rows
+                float* const tops = reinterpret_cast<float*>(lds + 2 * Z::BUF);
+                tops[w * 64 + lane] = top;
+                __syncthreads();
+                top = fmaxf(top, tops[(w ^ 1) * 64 + lane]);
+            }
+            const int e = __builtin_amdgcn_frexp_expf(top);
+            qmul = fmaxf(__builtin_ldexpf(scale_l2, e), 1e-37f);   // (not 0: -inf * 0 of a hidden key would be NaN)
+#pragma unroll
+            for (int c = 0; c < DW / 16; ++c)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float y = __builtin_ldexpf(x[c][j], -e);
+                    const _Float16 hi = (_Float16)y;
+                    qh[c][j] = hi;
+                    ql[c][j] = (_Float16)(y - (float)hi);
+                }
         }
     }
 
@@ -236,10 +260,9 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
     for (int n = 0; n < DT32; ++n)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[n][e] = 0.f;
-    const float scale_l2 = a.scale * 1.44269504088896f;
     const float cap_l2 = a.softcap * 1.44269504088896f;
     const float inv_cap_l2 = CAP ? 1.0f / cap_l2 : 0.f;
-    const float fac = CAP ? 1.0f : scale_l2;                 // scores are kept unscaled; the soft-cap leaves them in log2 units
+    const float fac = CAP ? 1.0f : qmul;                 // scores are kept unscaled; the soft-cap leaves them in log2 units
 
     // ---- staging
     const uint32_t row_b = dr * Z::ES;
@@ -366,7 +389,7 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
 #pragma unroll
             for (int b = 0; b < NB; ++b)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) sc[b][e] = paged_softcap_l2(sc[b][e] * scale_l2, cap_l2, inv_cap_l2);
+                for (int e = 0; e < 16; ++e) sc[b][e] = paged_softcap_l2(sc[b][e] * qmul, cap_l2, inv_cap_l2);
         }
         if (masked) {
             // key in [lo, pos] as one unsigned comparison against their number; a key among the first tokens as another
