@@ -851,3 +851,22 @@ def test_tiny_and_huge_queries_keep_their_accuracy(d, dtype, decode):
         err = (o.cpu().double() - ref).abs().max().item()
         print(f"{size:.3g} {softcap}: {err:.3g} of {tol:.3g}", flush=True)
         assert err <= tol
+
+
+@CALL
+def test_windows_of_any_size_do_not_wrap(decode):
+    pool = Pool(F16, 2, 64, 16, [200, 33])
+    q_len = [1, 1] if decode else [90, 33]
+    top = 2 ** 32 - 1
+    full = check_attention(pool, 4, q_len, decode=decode)[1]
+    for window, sink in ((top, 0), (top, top), (1, top), (0, top), (top - 1, 5)):
+        o = check_attention(pool, 4, q_len, decode=decode, window=window, sink=sink)[1]
+        assert (o - full).abs().max() < 1e-5
+
+
+@pytest.mark.parametrize("dtype, io", [(F8, torch.float16), (F16, torch.float16), (F8, torch.float32)])
+@pytest.mark.parametrize("window", [100, 384, 700, 1536, 1600])
+def test_windows_around_the_choice_of_wavefronts(dtype, io, window):
+    # chunks that fill blocks of 256 rows: four or eight wavefronts by the window
+    pool = Pool(dtype, 1, 128, 64, [2300, 700])
+    check_attention(pool, 4, [2300, 600], io, window=window, sink=0 if window in (384, 1536) else 3)

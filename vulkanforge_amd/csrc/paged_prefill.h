@@ -651,7 +651,12 @@ hipError_t launch_dim(const PagedAttnLaunch& L, hipStream_t stream) {
         // 160 / 172 us, 2 048 76 / 65 us, 1 024 tokens over 5 000 keys 102 / 110 us; F16 rows of 256: 8 192 tokens 753 / 1 012 us,
         // 4 096 327 / 271 us, 2 048 over 6 000 keys 301 / 356 us.)
         const uint64_t rows = (uint64_t)L.s.n_tokens * (L.n_heads / L.c.n_kv_heads);
-        const bool many = rows >= 256ull * L.s.n_seqs && (blocks_alike(L) || rows / 256u * L.c.n_kv_heads >= 512u);
+        // Short windows, rows of up to 128: two workgroups of four on a CU, one of which begins or ends a block while the other
+        // computes.  (Eight / four: FP8 / f16 rows, 2 x 4 096 tokens, window 128 92.5 / 78.5 us, 4 096, window 512 71.7 / 66.2, 8 192, window 1 024 202 / 187,
+        // 4 096 over 16 384, window 4 096 304 / 317; F16 pages 97.8 / 88.5, 74.3 / 72.9, 211 / 209, 320 / 352; FP8 / f32 rows 109 / 99,
+        // 90 / 92, 289 / 280, 479 / 500.)
+        const bool brief = d <= 128u && L.window != 0u && (uint64_t)L.window + L.n_sink <= (DT == kF8 && IOF16 ? 1536u : 384u);
+        const bool many = !brief && rows >= 256ull * L.s.n_seqs && (blocks_alike(L) || rows / 256u * L.c.n_kv_heads >= 512u);
         constexpr int CK = IOF16 ? 64 : 32, KT = 64;
         if (d <= 64u) return many ? launch_pre<DT, 64, IOF16, CAP, 64, 64, 8, 2>(L, stream) : launch_pre<DT, 64, IOF16, CAP, 64, 64, 4, 2>(L, stream);
         if (d <= 128u) return many ? launch_pre<DT, 128, IOF16, CAP, KT, CK, 8, 2>(L, stream) : launch_pre<DT, 128, IOF16, CAP, KT, CK, 4, 2>(L, stream);
