@@ -17,7 +17,7 @@
 //     F32 caches use the f32 matrix instruction.
 //   - The running maximum is only raised when a score exceeds it by 2^8; weights are kept times 2^6 (see paged_decode.hip).
 // Measured (f16 product of 8 192 x 8 192 matrices in the library: 1 175 TFLOP/s): 8 192 tokens from position 0, FP8, f16 rows,
-// 32 / 8 / 128: 565-585 us = 940-974 TFLOP/s, the matrix units busy 0.41 and the vector units 0.39 of the time (LDS 0.31): the two
+// 32 / 8 / 128: 565-620 us by card = 890-974 TFLOP/s, the matrix units busy 0.41 and the vector units 0.39 of the time (LDS 0.31): the two
 // wavefronts of a SIMD meet at the tile's barrier, so half of what could overlap does.  512 tokens over 4 096 keys, f32 rows: 81-83 us =
 // 450 TFLOP/s of useful work, 900 with the remainder products.  Windows of 1 024 keys: 560-575 TFLOP/s (18 tiles per block do not
 // hide a block's beginning and end).  Tried and not kept: two row blocks per wavefront (one wavefront per SIMD, 461 TFLOP/s: the
