@@ -870,3 +870,43 @@ def test_windows_around_the_choice_of_wavefronts(dtype, io, window):
     # chunks that fill blocks of 256 rows: four or eight wavefronts by the window
     pool = Pool(dtype, 1, 128, 64, [2300, 700])
     check_attention(pool, 4, [2300, 600], io, window=window, sink=0 if window in (384, 1536) else 3)
+
+
+@IOS
+@pytest.mark.parametrize("dtype", [F16, F8])
+def test_wide_rows_captured(dtype, io):
+    """Captured decode and prefill over rows of 512, replayed with other lengths, against the eager calls."""
+    pool = Pool(dtype, 2, 512, 16, [700, 90, 33], spare=0)
+    fwd = vf.PagedForward(pool.cache, 8)
+    off = torch.tensor([0, 20, 21, 50], dtype=torch.int32, device=DEV)
+    kv, table = pool.kv_dev.clone(), pool.table_dev.clone()
+    chunk, step = vf.SeqBatch(table, kv, off, n_tokens=50), vf.SeqBatch(table, kv)
+    q, q1 = rand_q(50, 8, 512, io), rand_q(3, 8, 512, io)
+    o, o1 = torch.zeros_like(q), torch.zeros_like(q1)
+
+    def calls(a, b):
+        fwd.prefill_attention(0, chunk, q, a)
+        fwd.decode_attention(0, step, q1, b)
+
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        calls(o, o1)
+    for rep, lens in enumerate(([700, 90, 33], [20, 90, 0], [699, 1, 33], [512, 64, 32])):
+        kv.copy_(torch.tensor(lens, dtype=torch.int32))
+        q.copy_(rand_q(50, 8, 512, io, seed=rep))
+        graph.replay()
+        eager, eager1 = torch.zeros_like(o), torch.zeros_like(o1)
+        calls(eager, eager1)
+        torch.cuda.synchronize()
+        assert torch.equal(o, eager) and torch.equal(o1, eager1) and bool(o.isfinite().all())
+
+
+@pytest.mark.parametrize("dtype", [F16, F8])
+def test_wide_rows_around_the_ways_of_dealing(dtype):
+    # a workgroup per sequence up to 256 keys, from 128 workgroups on up to 1 024; dealt beyond
+    for n in (255, 256, 257):
+        check_attention(Pool(dtype, 1, 512, 16, [n, 1, 17]), 2, [1] * 3, decode=True, max_kv_len=n)
+    for n in (1024, 1040):
+        kv = [n] + [5 + 3 * i % 70 for i in range(127)]
+        check_attention(Pool(dtype, 1, 512, 16, kv), 2, [1] * 128, decode=True, max_kv_len=n)
