@@ -596,7 +596,8 @@ int vfkv_paged_qk_rope_kv_write(vfkv_pages* c, uint32_t layer, const vfkv_seq_ba
  * (window == 0 or j > p - window or j < n_sink): a sliding window behind a few first tokens that stay visible.  A query
  * that sees nothing gets zeros.  What a query does not see has no part in its output, whatever bits the rows hold (NaN, infinities);
  * a row it does see enters by the formula, but an infinite element of K counts as NaN and one of V gives an infinity or NaN.
- * Over FP8 and F16 pages f32 queries enter the products as two f16 terms, an element exact to 2^-22 of the largest of its row.
+ * Over FP8 and F16 pages f32 queries enter the products as two f16 terms, an element exact to 2^-22 of the largest of its row, and so
+ * do the weights, whatever the type of q and o.
  * |q| * scale must stay below 2^126.  Elements of V in F32 pages must stay below 2^110: weights are kept up to 2^14 until the end. */
 typedef struct vfkv_paged_attn_params {
     uint32_t n_heads;

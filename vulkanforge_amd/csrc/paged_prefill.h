@@ -12,9 +12,9 @@
 //     scalar load two tiles ahead.
 //   - S^T = K Q^T and O^T += V^T P^T on v_mfma_f32_32x32x16_f16: the scores of a row stay in one lane and its opposite half, P is
 //     already where the second product wants it, V^T comes from the transposing LDS read.
-//   - f16 queries enter as they are and the weights as f16 (half a step of 2^-11 per weight, like the output's own rounding).  f32
-//     queries enter as f16 value + remainder, and so do the weights: f32-level accuracy for twice the products.
-//     F32 caches use the f32 matrix instruction.
+//   - f16 queries enter as they are, f32 queries as f16 value + remainder, and the weights as value + remainder for both: f32-level
+//     accuracy for one product more.  (Weights rounded to f16 are off by up to 2^-11 each, which large elements of V that cancel turn into
+//     ten steps of an f16 output.)  F32 caches use the f32 matrix instruction.
 //   - The running maximum is only raised when a score exceeds it by 2^8; weights are kept times 2^6 (see paged_decode.hip).
 // Measured (f16 product of 8 192 x 8 192 matrices in the library: 1 175 TFLOP/s): 8 192 tokens from position 0, FP8, f16 rows,
 // 32 / 8 / 128: 565-620 us by card = 890-974 TFLOP/s, the matrix units busy 0.41 and the vector units 0.39 of the time (LDS 0.31): the two
@@ -106,7 +106,7 @@ template <int DT, int D, bool IOF16, bool CAP, int KT, int CK, int NW, int MINW,
 __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnLaunch a, uint32_t n_split) {
     using Z = PreShape<DT, D, KT, NW>;
     constexpr bool F32C = DT == kF32;
-    constexpr bool PAIR = !IOF16 && !F32C;                   // queries and weights as value + remainder
+    constexpr bool QPAIR = !IOF16 && !F32C;                  // queries as value + remainder
     constexpr int NB = CK / 32;                              // 32-key blocks per chunk: what a wavefront takes through both products at once
     constexpr int DW = D / DS;                               // columns of a wavefront: DS wavefronts share 32 rows
     constexpr int DT32 = DW / 32;
@@ -186,7 +186,7 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
         tok += t0;
     }
     // ---- Q^T operands
-    half8_t qh[F32C ? 1 : DW / 16], ql[PAIR ? DW / 16 : 1];
+    half8_t qh[F32C ? 1 : DW / 16], ql[QPAIR ? DW / 16 : 1];
     float qf[F32C ? D / 2 : 1];
     const float scale_l2 = a.scale * 1.44269504088896f;
     float qmul = scale_l2;                                   // of the scores, to log2 units
@@ -378,7 +378,7 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
                 for (int c = 0; c < DW / 16; ++c) {
                     const half8_t k = *reinterpret_cast<const half8_t*>(krow + 32 * c);
                     sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[c], sc[b], 0, 0, 0);
-                    if constexpr (PAIR) sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[c], sc[b], 0, 0, 0);
+                    if constexpr (QPAIR) sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[c], sc[b], 0, 0, 0);
                 }
             }
         }
@@ -432,7 +432,7 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 sc[b][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][e], fac, -m));
-                if constexpr (F32C || PAIR) l += sc[b][e];
+                l += sc[b][e];
             }
         if constexpr (F32C) {
 #pragma unroll
@@ -455,20 +455,17 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float p0 = sc[kk / 2][8 * (kk % 2) + 2 * i], p1 = sc[kk / 2][8 * (kk % 2) + 2 * i + 1];
-                    const half2_t hh = half2_t{(_Float16)p0, (_Float16)p1};
-                    h[i] = __builtin_bit_cast(uint32_t, hh);
-                    // f16 weights: the sum is that of the weights as the product uses them, so their rounding cancels in the mean
-                    if constexpr (!PAIR) l = __builtin_amdgcn_fdot2(hh, half2_t{(_Float16)1.f, (_Float16)1.f}, l, false);
-                    if constexpr (PAIR) r[i] = pack_f16_remainder(p0, p1, h[i]);
+                    h[i] = __builtin_bit_cast(uint32_t, half2_t{(_Float16)p0, (_Float16)p1});
+                    r[i] = pack_f16_remainder(p0, p1, h[i]);
                 }
-                const half8_t ph = __builtin_bit_cast(half8_t, h);
+                const half8_t ph = __builtin_bit_cast(half8_t, h), pl = __builtin_bit_cast(half8_t, r);
 #pragma unroll
                 for (int n = 0; n < DT32; ++n) {
                     const half4_t v0 = lds_read_tr16(reinterpret_cast<const _Float16*>(vlane + 16 * kk * Z::VPITCH + 64 * n));
                     const half4_t v1 = lds_read_tr16(reinterpret_cast<const _Float16*>(vlane + (16 * kk + 8) * Z::VPITCH + 64 * n));
                     const half8_t v = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
                     acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph, acc[n], 0, 0, 0);
-                    if constexpr (PAIR) acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(half8_t, r), acc[n], 0, 0, 0);
+                    acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl, acc[n], 0, 0, 0);
                 }
             }
         }
