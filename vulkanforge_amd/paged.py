@@ -177,6 +177,8 @@ class PagedKvCache:
     def fork(self, pages: Sequence[int], kv_len: int, n_forks: int, stream=None) -> np.ndarray:
         """Page lists [n_forks, pages] of continuations of the sequence of ``kv_len`` positions in ``pages``: full pages
         are shared, a last page that is not full is copied into a page of the fork's own."""
+        if not 0 <= kv_len <= 0xFFFFFFFF or not 0 <= n_forks <= 0xFFFFFFFF:
+            raise ValueError(f"kv_len and n_forks must be between 0 and 2^32 - 1 (got {kv_len} and {n_forks})")
         used = self.pages_for(kv_len)
         p = _pages(pages)
         if len(p) < used:
