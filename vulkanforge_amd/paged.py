@@ -19,6 +19,12 @@ from .forward import Workspace
 from .kv_cache import KvDtype
 
 NO_PAGE = -1     # an entry of a page list or page table without a page
+_TOP = 0xFFFFFFFF
+
+
+def _fit(v: int) -> int:
+    """``v``, or 2^32 - 1 where ctypes would wrap it to another number: no layer, page, size or count may be that one."""
+    return v if 0 <= v <= _TOP else _TOP
 
 
 @dataclass
@@ -91,8 +97,8 @@ class PagedKvCache:
         L = _ffi.lib()
         self.config = config
         self.kv_dtype = KvDtype(config.dtype)
-        cfg = _ffi.PagesConfig(config.n_layers, config.n_kv_heads, config.head_dim, config.page_size, config.n_pages,
-                               int(config.dtype))
+        cfg = _ffi.PagesConfig(*(_fit(x) for x in (config.n_layers, config.n_kv_heads, config.head_dim, config.page_size,
+                                                   config.n_pages)), int(self.kv_dtype))
         handle = C.c_void_p()
         if layout_only or k_buffer or v_buffer:
             _ffi.check(L.vfkv_pages_create_external(C.byref(cfg), k_buffer or None, v_buffer or None, C.byref(handle)))
@@ -136,7 +142,7 @@ class PagedKvCache:
         return int(_ffi.lib().vfkv_pages_bytes_per_buffer(self._h))
 
     def offset_bytes(self, layer: int, page: int) -> int:
-        return int(_ffi.lib().vfkv_pages_offset_bytes(self._h, layer, page))
+        return int(_ffi.lib().vfkv_pages_offset_bytes(self._h, _fit(layer), _fit(page)))
 
     def pages_for(self, kv_len: int) -> int:
         """Pages a sequence of ``kv_len`` positions occupies."""
@@ -148,11 +154,12 @@ class PagedKvCache:
         return int(_ffi.lib().vfkv_pages_free_count(self._h))
 
     def refcount(self, page: int) -> int:
-        return int(_ffi.lib().vfkv_pages_refcount(self._h, page & 0xFFFFFFFF))
+        return int(_ffi.lib().vfkv_pages_refcount(self._h, _fit(page)))
 
     def alloc(self, n: int) -> List[int]:
         """The ``n`` lowest free pages; raises when fewer are free."""
-        out = np.empty(max(n, 1), np.uint32)
+        n = n if 0 <= n <= self.config.n_pages else _TOP                     # (more than there can be: the call says so)
+        out = np.empty(n if 0 < n < _TOP else 1, np.uint32)
         _ffi.check(_ffi.lib().vfkv_pages_alloc(self._h, n, _addr(out)))
         return out[:n].tolist()
 
@@ -177,7 +184,7 @@ class PagedKvCache:
     def fork(self, pages: Sequence[int], kv_len: int, n_forks: int, stream=None) -> np.ndarray:
         """Page lists [n_forks, pages] of continuations of the sequence of ``kv_len`` positions in ``pages``: full pages
         are shared, a last page that is not full is copied into a page of the fork's own."""
-        if not 0 <= kv_len <= 0xFFFFFFFF or not 0 <= n_forks <= 0xFFFFFFFF:
+        if not 0 <= kv_len <= _TOP or not 0 <= n_forks <= _TOP:
             raise ValueError(f"kv_len and n_forks must be between 0 and 2^32 - 1 (got {kv_len} and {n_forks})")
         used = self.pages_for(kv_len)
         p = _pages(pages)
@@ -243,7 +250,8 @@ class MRope:
         if not 1 <= len(sections) <= 4:
             raise ValueError("1 to 4 axes")
         self.n_axes = len(sections)
-        self._args = _ffi.MRopeParams(rope_mode, rotary_dim, self.n_axes, int(interleaved),
+        sections = [_fit(x) for x in sections]
+        self._args = _ffi.MRopeParams(_fit(rope_mode), _fit(rotary_dim), self.n_axes, _fit(int(interleaved)),
                                       (C.c_uint32 * 4)(*(sections + [0] * (4 - self.n_axes))), freq_base, freq_scale,
                                       attn_factor, eps)
         self.args = C.byref(self._args)
@@ -254,7 +262,7 @@ class PagedWorkspace(Workspace):
 
     def __init__(self, cache: PagedKvCache, n_heads: int):
         h = C.c_void_p()
-        _ffi.check(_ffi.lib().vfkv_paged_workspace_create(cache.handle, n_heads, C.byref(h)))
+        _ffi.check(_ffi.lib().vfkv_paged_workspace_create(cache.handle, _fit(n_heads), C.byref(h)))
         self._h = h
 
     @property
@@ -322,18 +330,20 @@ class PagedForward:
                            self._dev(positions, (rope.n_axes, batch.n_tokens), "torch.int32", batch, "positions"),
                            self._dev(freq_factors, (half,), "torch.float32", batch, "freq_factors"),
                            self.n_heads, io, qs or 0, os_ or 0, ks, vs)
-        _ffi.check(_ffi.lib().vfkv_paged_qk_rope_kv_write(self.cache.handle, layer, batch.args, C.byref(r), rope.args,
+        _ffi.check(_ffi.lib().vfkv_paged_qk_rope_kv_write(self.cache.handle, _fit(layer), batch.args, C.byref(r), rope.args,
                                                           _stream(stream, batch.index)))
 
     def _attention(self, fn, layer, batch, q, o, window, n_sink, scale, softcap, stream) -> None:
+        if window < 0 or n_sink < 0:
+            raise ValueError("window and n_sink must not be negative")
+        if window > _TOP or n_sink > _TOP:                   # (every length is below 2^31: more is the same as the most)
+            window, n_sink = min(window, _TOP), min(n_sink, _TOP)
         qp, qs, io = self._rows(q, self.n_heads, batch, "q")
         op, os_, ioo = self._rows(o, self.n_heads, batch, "o")
         if io != ioo:
             raise ValueError("q and o must have one dtype")
-        if window < 0 or n_sink < 0:
-            raise ValueError("window and n_sink must not be negative")
         p = _ffi.PagedAttnParams(self.n_heads, window, n_sink, io, qs, os_, self.attn_scale if scale is None else scale, softcap)
-        _ffi.check(fn(self.cache.handle, layer, batch.args, C.byref(p), qp, op, self.workspace.handle, _stream(stream, batch.index)))
+        _ffi.check(fn(self.cache.handle, _fit(layer), batch.args, C.byref(p), qp, op, self.workspace.handle, _stream(stream, batch.index)))
 
     def decode_attention(self, layer: int, batch: SeqBatch, q, o, window: int = 0, n_sink: int = 0,
                          scale: Optional[float] = None, softcap: float = 0.0, stream=None) -> None:
