@@ -532,9 +532,10 @@ int vfkv_pages_compact(vfkv_pages* c, uint32_t* new_ids_out, vfkv_stream stream)
 /* A batch of sequences.  The three arrays are DEVICE arrays, read when the work runs, so a captured call follows them from replay
  * to replay.  Sequence s owns the token rows [q_offsets[s], q_offsets[s + 1]) of q / k / v / o (q_offsets NULL:
  * n_tokens == n_seqs, row s); they are its last positions: row i of m has position kv_lens[s] - m + i, and
- * kv_lens[s] counts them.  Values the kernels cannot use are bounded, never followed: kv_lens are clamped to
- * [0, min(table_stride * page_size, 2^23)], q_offsets to [0, n_tokens]; a page table entry outside [0, n_pages) has no rows (writes to it
- * are dropped, its keys are invisible), a token at a negative position has neither row nor visible keys.
+ * kv_lens[s] counts them.  Values the kernels cannot use are bounded, never followed: negative kv_lens count as 0, q_offsets are clamped to
+ * [0, n_tokens]; a page table entry outside [0, n_pages) has no rows (writes to it are dropped, its keys are invisible), a token at a
+ * negative position has neither row nor visible keys.  A position from min(table_stride * page_size, 2^23) on has no row either: the
+ * write drops it (and turns its query as any other), the attention calls clamp kv_lens to that length.
  * Rows of no sequence (n_tokens may exceed q_offsets[n_seqs]) are left as they were. */
 typedef struct vfkv_seq_batch {
     const int32_t* page_table; /* [n_seqs][table_stride] */

@@ -88,6 +88,11 @@ __device__ __forceinline__ float paged_softcap_l2(float y, float cap_l2, float i
     const float far = __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(t + 1.0f), 1.0f);
     return copysignf(cap_l2 * (x < 0.8f ? near : far), y);
 }
+// Length of sequence s as given, not negative: what positions are counted from.  (A position the page table cannot hold has no row.)
+__device__ __forceinline__ uint32_t paged_given_len(const PagedSeqs& S, uint32_t s) {
+    const int32_t n = S.kv_lens[s];
+    return n < 0 ? 0u : (uint32_t)n;
+}
 // Length of sequence s, within what its page table can hold.
 __device__ __forceinline__ uint32_t paged_kv_len(const PagedSeqs& S, uint32_t s) {
     const int32_t n = S.kv_lens[s];
