@@ -534,8 +534,8 @@ int vfkv_pages_compact(vfkv_pages* c, uint32_t* new_ids_out, vfkv_stream stream)
  * n_tokens == n_seqs, row s); they are its last positions: row i of m has position kv_lens[s] - m + i, and
  * kv_lens[s] counts them.  Values the kernels cannot use are bounded, never followed: negative kv_lens count as 0, q_offsets are clamped to
  * [0, n_tokens]; a page table entry outside [0, n_pages) has no rows (writes to it are dropped, its keys are invisible), a token at a
- * negative position has neither row nor visible keys.  A position from min(table_stride * page_size, 2^23) on has no row either: the
- * write drops it (and turns its query as any other), the attention calls clamp kv_lens to that length.
+ * negative position has neither row nor visible keys.  Positions from min(table_stride * page_size, 2^23) on have no rows
+ * either; their queries are turned by their angles and see what the rules below leave of the keys in front of that.
  * Rows of no sequence (n_tokens may exceed q_offsets[n_seqs]) are left as they were. */
 typedef struct vfkv_seq_batch {
     const int32_t* page_table; /* [n_seqs][table_stride] */

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import vulkanforge_amd as vf
+from paged_exact import assert_near, exact
 from paged_ref import DEV, Pool, turned
 
 pytestmark = pytest.mark.gpu
@@ -111,3 +112,74 @@ def test_captured_step_replayed_past_its_table_leaves_shared_pages_alone():
     torch.cuda.synchronize()
     assert torch.equal(kb, full[0]) and torch.equal(vb, full[1])
     assert float(kb[0, first].abs().max()) == 0.0 and [float(kb[0, x[2], 0, j, 0]) for x in lists for j in (0, 15)] == [1.0, 16.0] * 2
+
+
+@pytest.mark.parametrize("decode", [True, False])
+@pytest.mark.parametrize("dtype, d", [(F16, 64), (F8, 128), (F32, 128), (F8, 40), (F32, 256), (F16, 512), (F16, 256)])
+@pytest.mark.parametrize("window, sink", [(0, 0), (20, 0), (40, 5), (100, 64), (7, 130), (1, 0)])
+def test_queries_beyond_the_table_see_what_is_in_front_of_its_end(decode, dtype, d, window, sink):
+    """Positions count from the length as given, so a window moves on when the keys do not."""
+    page = 16
+    pool = Pool(dtype, 2, d, page, [176, 64, 16, 176, 176, 176, 176], spare=1, extra_entries=0)    # (176: not a multiple of any tile)
+    lens = [177, 70, 16, 190, 176 + 45, 5000, 2 ** 31 - 1]
+    pool.kv_dev.copy_(torch.tensor(lens, dtype=torch.int32))
+    q_len = [1] * 7 if decode else [9, 70, 3, 60, 100, 2, 1]
+    n = sum(q_len)
+    for io in (torch.float32, torch.float16):
+        q = torch.randn((n, 8, d), generator=torch.Generator().manual_seed(d)).to(io).to(DEV)
+        o = torch.full_like(q, float("nan"))
+        fwd = vf.PagedForward(pool.cache, 8)
+        (fwd.decode_attention if decode else fwd.prefill_attention)(0, pool.batch(None if decode else q_len), q, o, window=window, n_sink=sink)
+        torch.cuda.synchronize()
+        ref, bound = exact(pool, q, q_len, window, sink, lens=lens)
+        assert_near(o, ref, bound, io)
+
+
+@pytest.mark.parametrize("dtype, d, io", [(F16, 64, torch.float32), (F8, 64, torch.float16), (F8, 128, torch.float16), (F16, 256, torch.float16)])
+@pytest.mark.parametrize("window", [0, 50])
+def test_blocks_of_256_rows_across_the_end_of_the_table(dtype, d, io, window):
+    pool = Pool(dtype, 1, d, 16, [1040], spare=1, extra_entries=0)
+    q = torch.randn((400, 4, d), generator=torch.Generator().manual_seed(d)).to(io).to(DEV)
+    for length in (1041, 1100, 1240, 1439, 1440, 1600):
+        pool.kv_dev.fill_(length)
+        o = torch.full_like(q, float("nan"))
+        vf.PagedForward(pool.cache, 4).prefill_attention(0, pool.batch([400]), q, o, window=window, n_sink=window // 10)
+        torch.cuda.synchronize()
+        ref, bound = exact(pool, q, [400], window, window // 10, lens=[length])
+        assert_near(o, ref, bound, io, length)
+
+
+@pytest.mark.parametrize("decode", [True, False])
+def test_long_tables_and_lengths_beyond_them_in_parts(decode):
+    pool = Pool(F8, 1, 128, 64, [5120, 64], spare=1, extra_entries=0)
+    lens = [5300, 5120 + 3]
+    pool.kv_dev.copy_(torch.tensor(lens, dtype=torch.int32))
+    q_len = [1, 1] if decode else [7, 3]
+    for window, sink in ((0, 0), (2000, 70), (150, 1)):
+        q = torch.randn((sum(q_len), 4, 128), generator=torch.Generator().manual_seed(window)).to(DEV)
+        o = torch.full_like(q, float("nan"))
+        fwd = vf.PagedForward(pool.cache, 4)
+        (fwd.decode_attention if decode else fwd.prefill_attention)(0, pool.batch(None if decode else q_len), q, o, window=window, n_sink=sink)
+        torch.cuda.synchronize()
+        ref, bound = exact(pool, q, q_len, window, sink, lens=lens)
+        assert_near(o, ref, bound, torch.float32)
+
+
+@pytest.mark.parametrize("dtype, d", [(F16, 64), (F8, 128), (F32, 64)])
+def test_rows_behind_the_end_of_the_table_do_not_reach_the_output(dtype, d):
+    """The tile that the table's end cuts: what lies in the last page behind it is not there, whatever it holds."""
+    pool = Pool(dtype, 1, d, 16, [48], spare=1, extra_entries=0)
+    bad = float("nan")
+    last = int(pool.table[0, 2])
+    q = torch.randn((90, 2, d), generator=torch.Generator().manual_seed(1)).to(DEV)
+    other = [p for p in range(pool.k.shape[1]) if p not in pool.table[0].tolist()]
+    for x in (pool.k, pool.v):
+        x[0, other] = torch.full_like(x[0, other].float(), bad).to(x.dtype)
+    for length in (49, 64, 90, 120):
+        pool.kv_dev.fill_(length)
+        o = torch.full_like(q, float("nan"))
+        vf.PagedForward(pool.cache, 2).prefill_attention(0, pool.batch([90]), q, o)
+        torch.cuda.synchronize()
+        ref, bound = exact(pool, q, [90], lens=[length])
+        assert last < pool.k.shape[1]
+        assert_near(o, ref, bound, torch.float32, length)

@@ -22,7 +22,7 @@ struct PagedSeqs {
     const int32_t* kv_lens;    // [n_seqs]
     const int32_t* q_offsets;  // [n_seqs + 1] or NULL: token t is the one token of sequence t
     uint32_t n_seqs, table_stride, n_tokens;
-    uint32_t limit;            // min(table_stride * page_size, kPagedMaxLen): longest length the kernels follow
+    uint32_t limit;            // min(table_stride * page_size, kPagedMaxLen): positions from here on have no row
 };
 struct PagedAttnLaunch {
     PagedSlab c;
@@ -88,15 +88,11 @@ __device__ __forceinline__ float paged_softcap_l2(float y, float cap_l2, float i
     const float far = __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(t + 1.0f), 1.0f);
     return copysignf(cap_l2 * (x < 0.8f ? near : far), y);
 }
-// Length of sequence s as given, not negative: what positions are counted from.  (A position the page table cannot hold has no row.)
-__device__ __forceinline__ uint32_t paged_given_len(const PagedSeqs& S, uint32_t s) {
-    const int32_t n = S.kv_lens[s];
-    return n < 0 ? 0u : (uint32_t)n;
-}
-// Length of sequence s, within what its page table can hold.
+// Length of sequence s as given, not negative: what positions are counted from.  It may pass S.limit: positions from there on have no
+// row, so whoever turns one into a table entry compares it first.
 __device__ __forceinline__ uint32_t paged_kv_len(const PagedSeqs& S, uint32_t s) {
     const int32_t n = S.kv_lens[s];
-    return n < 0 ? 0u : (uint32_t)n < S.limit ? (uint32_t)n : S.limit;
+    return n < 0 ? 0u : (uint32_t)n;
 }
 // Token rows [lo, hi) of sequence s.
 __device__ __forceinline__ void paged_rows(const PagedSeqs& S, uint32_t s, uint32_t& lo, uint32_t& hi) {

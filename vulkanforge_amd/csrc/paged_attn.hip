@@ -28,13 +28,14 @@ __global__ __launch_bounds__(256) void paged_generic_kernel(PagedAttnLaunch a) {
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     float m = kMasked, l = 0.f;
     if (pos >= 0) {
-        const uint32_t p = (uint32_t)pos, lo = paged_window_lo(a.window, p);
-        const uint32_t sink = a.n_sink < lo ? a.n_sink : lo;
+        // keys up to the query's own, as far as the table has rows
+        const uint32_t end = (uint32_t)pos < a.s.limit ? (uint32_t)pos + 1u : a.s.limit, wlo = paged_window_lo(a.window, (uint32_t)pos);
+        const uint32_t lo = wlo < end ? wlo : end, sink = a.n_sink < lo ? a.n_sink : lo;
         // chunks of the first tokens, then chunks of the window
-        const uint32_t nsc = (sink + 63u) / 64u, nwc = (p + 1u - lo + 63u) / 64u;
+        const uint32_t nsc = (sink + 63u) / 64u, nwc = (end - lo + 63u) / 64u;
         for (uint32_t c = 0; c < nsc + nwc; ++c) {
             const uint32_t j = c < nsc ? c * 64u + (uint32_t)lane : lo + (c - nsc) * 64u + (uint32_t)lane;
-            bool seen = c < nsc ? j < sink : j <= p;
+            bool seen = c < nsc ? j < sink : j < end;
             uint64_t row = 0u;                                       // byte offset of the key's row
             if (seen) {
                 const uint32_t page = paged_page(a.c, a.s, s, j >> a.c.page_shift);

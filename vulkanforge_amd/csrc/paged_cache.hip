@@ -172,7 +172,7 @@ __global__ __launch_bounds__(kWriteWaves * kWave) void paged_write_quads_kernel(
     uint32_t r0, r1;
     paged_rows(a.s, s, r0, r1);
     if (tok < r0 || tok >= r1) return;
-    const int64_t pos = (int64_t)paged_given_len(a.s, s) - (int64_t)(r1 - tok);
+    const int64_t pos = (int64_t)paged_kv_len(a.s, s) - (int64_t)(r1 - tok);
     const uint32_t page = pos >= 0 && pos < (int64_t)a.s.limit ? paged_page(a.c, a.s, s, (uint32_t)pos >> a.c.page_shift) : a.c.n_pages;
     const uint32_t slot = (uint32_t)pos & ((1u << a.c.page_shift) - 1u);
     const uint64_t page_at = (uint64_t)(page < a.c.n_pages ? page : 0u) * a.c.page_bytes;
@@ -278,7 +278,7 @@ __global__ __launch_bounds__(kWriteWaves * kWave) void paged_write_kernel(PagedW
     if (s >= a.s.n_seqs) return;                                  // a padding row: left as it was
     uint32_t r0, r1;
     paged_rows(a.s, s, r0, r1);
-    const int64_t pos = (int64_t)paged_given_len(a.s, s) - (int64_t)(r1 - tok);
+    const int64_t pos = (int64_t)paged_kv_len(a.s, s) - (int64_t)(r1 - tok);
     const uint32_t D = a.c.head_dim, half = a.rotary_dim / 2u;
     const uint32_t nq = a.q ? a.n_heads : 0u, hkv = a.c.n_kv_heads;
     if (blockIdx.y * kWriteWaves < nq + hkv) {

@@ -61,15 +61,16 @@ struct DecShape {
     static constexpr bool ONE = D == 512;
 };
 
-// Units of a sequence of n keys: first tokens, then the window of the query at position n - 1.
+// Units of a sequence: first tokens, then the window of the query at position len - 1, as far as there are rows (n keys).
 struct SeqUnits {
     uint32_t n, lo, sink, sink_units, first, units;
 };
-__device__ __forceinline__ SeqUnits seq_units(uint32_t n, uint32_t window, uint32_t n_sink, uint32_t uk_shift) {
-    const uint32_t uk = 1u << uk_shift;
+__device__ __forceinline__ SeqUnits seq_units(const PagedAttnLaunch& a, uint32_t len, uint32_t uk_shift) {
+    const uint32_t uk = 1u << uk_shift, n = len < a.s.limit ? len : a.s.limit, n_sink = a.n_sink;
+    const uint32_t lo = len ? paged_window_lo(a.window, len - 1u) : 0u;
     SeqUnits r;
     r.n = n;
-    r.lo = n ? paged_window_lo(window, n - 1u) : 0u;
+    r.lo = lo < n ? lo : n;
     r.sink = n_sink < r.lo ? n_sink : r.lo;
     r.first = r.lo >> uk_shift;
     const uint32_t su = (r.sink + uk - 1u) >> uk_shift;
@@ -112,7 +113,7 @@ __device__ __forceinline__ void unit_prefix(const PagedAttnLaunch& a, uint32_t* 
     uint32_t carry = 0u;
     for (uint32_t base = 0; base < a.s.n_seqs; base += 256u) {
         const uint32_t s = base + (uint32_t)tid;
-        uint32_t x = s < a.s.n_seqs ? line_units(seq_units(paged_kv_len(a.s, s), a.window, a.n_sink, SHIFT).units) : 0u;
+        uint32_t x = s < a.s.n_seqs ? line_units(seq_units(a, paged_kv_len(a.s, s), SHIFT).units) : 0u;
         const uint32_t mine = x;
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) {
@@ -162,7 +163,7 @@ __global__ __launch_bounds__(256, D >= 256 ? 1 : 2) void paged_decode_kernel(Pag
     if (direct) {
         s_first = wg;
         s_end = wg + 1u;
-        u1 = line_units(seq_units(__builtin_amdgcn_readfirstlane(paged_kv_len(a.s, wg)), a.window, a.n_sink, Z::SHIFT).units);
+        u1 = line_units(seq_units(a, __builtin_amdgcn_readfirstlane(paged_kv_len(a.s, wg)), Z::SHIFT).units);
         if (u1 == 0u) { no_keys(wg); return; }
     } else {
         unit_prefix<Z::SHIFT>(a, pre, wave_sum, tid);
@@ -211,7 +212,7 @@ __global__ __launch_bounds__(256, D >= 256 ? 1 : 2) void paged_decode_kernel(Pag
         const uint32_t ps = direct ? 0u : __builtin_amdgcn_readfirstlane(pre[s]), pe = direct ? u1 : __builtin_amdgcn_readfirstlane(pre[s + 1u]);
         if (ps >= u1) break;
         if (ps == pe) continue;
-        const SeqUnits Q = seq_units(__builtin_amdgcn_readfirstlane(paged_kv_len(a.s, s)), a.window, a.n_sink, Z::SHIFT);
+        const SeqUnits Q = seq_units(a, __builtin_amdgcn_readfirstlane(paged_kv_len(a.s, s)), Z::SHIFT);
         // this range's part of the sequence, units [ua, ub)
         const uint32_t la = (ps > u0 ? ps : u0) - ps, lb = (pe < u1 ? pe : u1) - ps;
         const uint32_t ua = la > kBegin ? la - kBegin : 0u, ub = lb > kBegin ? lb - kBegin : 0u;
@@ -560,12 +561,12 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnLaunch a, uin
     __shared__ float ls[256], ms[256];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const uint32_t head = blockIdx.x, s = blockIdx.y;
-    const uint32_t mine = line_units(seq_units(paged_kv_len(a.s, s), a.window, a.n_sink, uk_shift).units);
+    const uint32_t mine = line_units(seq_units(a, paged_kv_len(a.s, s), uk_shift).units);
     uint32_t before = 0u, U = mine;
     if (a.s.n_seqs > 1u) {
         uint32_t all = 0u;
         for (uint32_t t = tid; t < a.s.n_seqs; t += 256u) {
-            const uint32_t x = line_units(seq_units(paged_kv_len(a.s, t), a.window, a.n_sink, uk_shift).units);
+            const uint32_t x = line_units(seq_units(a, paged_kv_len(a.s, t), uk_shift).units);
             all += x;
             before += t < s ? x : 0u;
         }

@@ -152,9 +152,10 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
     const int kv_len = (int)__builtin_amdgcn_readfirstlane(paged_kv_len(a.s, s));
     const int pos0 = kv_len - (int)(t1 - t0);                // position of the chunk's first token
     const int pmin = pos0 + (int)(row0 / group), pmax = pos0 + (int)((row1 - 1u) / group);
-    // key tiles of the block: first tokens in front of the window of its first query, then up to its last query
-    const uint32_t n_keys = pmax < 0 ? 0u : (uint32_t)pmax + 1u;
-    const uint32_t lo_min = pmin > 0 ? paged_window_lo(a.window, (uint32_t)pmin) : 0u;
+    // key tiles of the block: first tokens in front of the window of its first query, then up to its last query, as far as there are rows
+    auto keys_to = [&](int pos) { return pos < 0 ? 0u : (uint32_t)pos < a.s.limit ? (uint32_t)pos + 1u : a.s.limit; };
+    const uint32_t n_keys = keys_to(pmax), all_see = keys_to(pmin);       // (every query sees up to all_see, its window aside)
+    const uint32_t wlo = pmin > 0 ? paged_window_lo(a.window, (uint32_t)pmin) : 0u, lo_min = wlo < n_keys ? wlo : n_keys;
     const uint32_t first = lo_min / KT;
     const uint32_t sink = a.n_sink < lo_min ? a.n_sink : lo_min;
     const uint32_t su = (sink + KT - 1u) / KT;
@@ -168,6 +169,7 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
     const bool wave_has = wr0 < row1;
     const uint32_t wr1 = row1 < wr0 + 32u ? row1 : wr0 + 32u;
     const int wmin = wave_has ? pos0 + (int)(wr0 / group) : 0, wmax = wave_has ? pos0 + (int)((wr1 - 1u) / group) : -1;
+    const int wave_sees = (int)keys_to(wmin);                // every query of the wavefront, its window aside
     const int wlo_max = wmax > 0 ? (int)paged_window_lo(a.window, (uint32_t)wmax) : 0;     // window start of the last query
     const int wlo_min = wmin > 0 ? (int)paged_window_lo(a.window, (uint32_t)wmin) : 0;
     uint32_t lo, span, lead;                     // a row sees the keys [lo, lo + span) and [0, lead)
@@ -180,9 +182,10 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
         tok = rr / group;
         head = kvh * group + rr - tok * group;
         const int pos = real ? pos0 + (int)tok : -1;
+        const uint32_t end = keys_to(pos);
         lo = pos > 0 ? paged_window_lo(a.window, (uint32_t)pos) : 0u;
-        span = pos < 0 ? 0u : (uint32_t)pos + 1u - lo;
-        lead = pos < 0 ? 0u : a.n_sink < (uint32_t)pos + 1u ? a.n_sink : (uint32_t)pos + 1u;
+        span = end > lo ? end - lo : 0u;
+        lead = a.n_sink < end ? a.n_sink : end;
         tok += t0;
     }
     // ---- Q^T operands
@@ -308,7 +311,7 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
         uint8_t* const kl = lds + buf * Z::BUF;
         uint8_t* const vl = kl + KT * Z::KPITCH;
         const uint32_t kb = tile_key(t);
-        const bool hidden = kb + KT > (uint32_t)(pmin < 0 ? 0 : pmin + 1) ||
+        const bool hidden = kb + KT > all_see ||
                             !(kb + KT <= a.n_sink || a.window == 0u || kb >= paged_window_lo(a.window, (uint32_t)pmax));
         bool part = hidden;
 #pragma unroll
@@ -497,7 +500,7 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
                     }
                     // (a chunk that none of the wavefront's queries sees is passed over)
                     const bool none = kb > wmax || ((uint32_t)kb >= a.n_sink && kb + CK <= wlo_min);
-                    auto masked = [&] { return !(kb + CK - 1 <= wmin && (kb >= wlo_max || (uint32_t)(kb + CK) <= a.n_sink) && !ghost); };
+                    auto masked = [&] { return !(kb + CK <= wave_sees && (kb >= wlo_max || (uint32_t)(kb + CK) <= a.n_sink) && !ghost); };
                     if constexpr (DS == 1) {
                         if (none) return;
                         float16_t sc[NB];
