@@ -78,6 +78,11 @@ uint32_t paged_decode_wgs(uint32_t head_groups);
 hipError_t launch_paged_generic(const PagedAttnLaunch& L, hipStream_t stream);
 
 #ifdef __HIPCC__
+// Running maximum of a row that has seen no key yet: below every score.
+constexpr float kNoScore = -3.40282347e38f;
+// A row is far out when its maximum (log2 units) leaves [-2^24, 2^24]: score * factor rounded once for the maximum and left exact
+// inside the multiply-add of a weight would differ by more than a unit of log2 there, and the weights leave their f16 range.
+__device__ __forceinline__ bool paged_far(float m) { return fabsf(m) > 16777216.f && m != kNoScore; }
 // Logit soft-cap in log2 units, cap * tanh(y / cap), to a few steps of f32 at every size: the truncated continued fraction of tanh
 // (7 / 5 terms, 8e-9 relative) below 0.8, 1 - 2 / (exp(2 x) + 1) on the hardware exponential and reciprocal above.  (The second alone
 // is off by 1e-7 absolute, which a cap of 50 turns into 5e-6 of a score.)

@@ -26,7 +26,7 @@ __global__ __launch_bounds__(256) void paged_generic_kernel(PagedAttnLaunch a) {
         q[d] = (float)reinterpret_cast<const T*>(a.q)[(uint64_t)tok * a.q_stride + (uint64_t)head * D + d] * a.scale;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    float m = kMasked, l = 0.f;
+    float m = kNoScore, l = 0.f;
     if (pos >= 0) {
         // keys up to the query's own, as far as the table has rows
         const uint32_t end = (uint32_t)pos < a.s.limit ? (uint32_t)pos + 1u : a.s.limit, wlo = paged_window_lo(a.window, (uint32_t)pos);
@@ -43,7 +43,7 @@ __global__ __launch_bounds__(256) void paged_generic_kernel(PagedAttnLaunch a) {
                 const uint32_t slot = j & ((1u << a.c.page_shift) - 1u);
                 if (seen) row = (uint64_t)page * a.c.page_bytes + (((uint64_t)kvh << a.c.page_shift) + slot) * D * es;
             }
-            float x = kMasked;
+            float x = kNoScore;
             if (seen) {
                 float dot = 0.f;
                 const uint8_t* const kp = a.c.k + row;

@@ -271,7 +271,8 @@ __global__ __launch_bounds__(256, D >= 256 ? 1 : 2) void paged_decode_kernel(Pag
         float4_t acc[Z::NT];
 #pragma unroll
         for (int n = 0; n < Z::NT; ++n) acc[n] = float4_t{0.f, 0.f, 0.f, 0.f};
-        float m = kMasked, l = 0.f;                                      // l: this lane's keys only, summed at the end
+        float m = kNoScore, l = 0.f;                                     // l: this lane's keys only, summed at the end
+        bool far = false;                                                // some row is far out: products are rounded before they are compared
 
         auto unit_key = [&](uint32_t u) { return (u < Q.sink_units ? u : Q.first + u - Q.sink_units) * (uint32_t)Z::UK; };
         auto get_pages = [&](uint32_t u) {
@@ -362,6 +363,14 @@ __global__ __launch_bounds__(256, D >= 256 ? 1 : 2) void paged_decode_kernel(Pag
 #pragma unroll
                     for (int i = 0; i < 4; ++i) x[t][i] = paged_softcap_l2(x[t][i] * fac, cap_l2, inv_cap_l2);
             }
+            auto round_products = [&] {
+                to_l2 = 1.0f;
+#pragma unroll
+                for (int t = 0; t < SUB; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[t][i] *= fac;
+            };
+            if (DT != kF32 && far) round_products();                     // (F32: fac is 1; far is never set with a soft-cap)
             if (!full) {
 #pragma unroll
                 for (int t = 0; t < SUB; ++t)
@@ -379,8 +388,13 @@ __global__ __launch_bounds__(256, D >= 256 ? 1 : 2) void paged_decode_kernel(Pag
             for (int t = 0; t < SUB; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) mx = fmaxf(mx, x[t][i]);
-            if (__any(mx * to_l2 > m + (kRaise + kBias))) {
-                const float mn = fmaxf(m, max_over_groups(mx) * to_l2 - kBias);
+            if (__any(mx * to_l2 - m > kRaise + kBias)) {
+                const float mn = fmaxf(m, max_over_groups(mx * to_l2) - kBias);
+                if (DT != kF32 && !(a.softcap > 0.f)) {
+                    const bool now = __any(paged_far(mn));
+                    if (now && !far) round_products();
+                    far = now;
+                }
                 const float corr = __builtin_amdgcn_exp2f(m - mn);
                 m = mn;
                 l *= corr;
@@ -593,7 +607,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnLaunch a, uin
     auto part_row = [&](uint32_t x) { return ((uint64_t)x * 2u + (x == wa ? slot_a : 0u)) * a.n_heads + head; };
     // eight parts at a time, maxima, sums and outputs requested together: one trip to memory for up to 8 * groups parts
     constexpr int AT_ONCE = 8;
-    float M = kMasked, L = 0.f;
+    float M = kNoScore, L = 0.f;
     float4_t sum = {0.f, 0.f, 0.f, 0.f};
     if (grp < groups) {
         for (uint32_t x0 = wa + grp; x0 <= wb; x0 += AT_ONCE * groups) {

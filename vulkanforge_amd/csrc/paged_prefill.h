@@ -258,7 +258,8 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
     }
 
     float16_t acc[DT32];
-    float m = kMasked, l = 0.f;                              // l: this lane's keys only, summed at the end
+    float m = kNoScore, l = 0.f;                             // l: this lane's keys only, summed at the end
+    uint32_t far = 0u;                                       // some row is far out: products are rounded before they are compared
 #pragma unroll
     for (int n = 0; n < DT32; ++n)
 #pragma unroll
@@ -394,6 +395,15 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
 #pragma unroll
                 for (int e = 0; e < 16; ++e) sc[b][e] = paged_softcap_l2(sc[b][e] * qmul, cap_l2, inv_cap_l2);
         }
+        float f = fac;
+        auto round_products = [&] {
+            f = 1.0f;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sc[b][e] *= fac;
+        };
+        if (!CAP && __builtin_expect(far != 0u, 0)) round_products();
         if (masked) {
             // key in [lo, pos] as one unsigned comparison against their number; a key among the first tokens as another
             auto hide = [&](auto firsts) {
@@ -420,8 +430,13 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
         for (int b = 0; b < NB; ++b)
 #pragma unroll
             for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[b][e]);
-        if (__any(mx * fac > m + (kRaise + kBias))) {
-            const float mn = fmaxf(m, max_over_halves(mx) * fac - kBias);
+        if (__any(mx * f - m > kRaise + kBias)) {
+            const float mn = fmaxf(m, max_over_halves(mx * f) - kBias);
+            if constexpr (!CAP) {
+                const uint32_t now = __builtin_amdgcn_readfirstlane(__any(paged_far(mn)) ? 1u : 0u);
+                if (__builtin_expect(now != 0u && far == 0u, 0)) round_products();
+                far = now;
+            }
             const float corr = __builtin_amdgcn_exp2f(m - mn);
             m = mn;
             l *= corr;
@@ -434,7 +449,7 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
         for (int b = 0; b < NB; ++b)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                sc[b][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][e], fac, -m));
+                sc[b][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][e], f, -m));
                 l += sc[b][e];
             }
         if constexpr (F32C) {

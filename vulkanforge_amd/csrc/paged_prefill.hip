@@ -17,7 +17,7 @@ __global__ __launch_bounds__(256) void paged_rows_merge_kernel(PagedAttnLaunch a
     bool mine = grp < rows_here * per_row && row < (uint64_t)a.s.n_tokens * a.n_heads;
     const uint32_t tok = mine ? (uint32_t)(row / a.n_heads) : 0u, head = mine ? (uint32_t)(row - (uint64_t)tok * a.n_heads) : 0u;
     mine = mine && paged_seq_of(a.s, tok) < a.s.n_seqs;
-    float M = kMasked, L = 0.f;
+    float M = kNoScore, L = 0.f;
     float4_t sum = {0.f, 0.f, 0.f, 0.f};
     if (mine) {
         constexpr int AT_ONCE = 8;
