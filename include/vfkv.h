@@ -596,10 +596,12 @@ int vfkv_paged_qk_rope_kv_write(vfkv_pages* c, uint32_t layer, const vfkv_seq_ba
  * What a query sees and how its scores are formed.  The query at position p sees key j when j <= p and
  * (window == 0 or j > p - window or j < n_sink): a sliding window behind a few first tokens that stay visible.  A query
  * that sees nothing gets zeros.  What a query does not see has no part in its output, whatever bits the rows hold (NaN, infinities);
- * a row it does see enters by the formula, but an infinite element of K counts as NaN and one of V gives an infinity or NaN.
+ * a row it does see enters by the formula, but an infinite element of K gives NaN or, where the score is minus infinity, no weight, and
+ * one of V gives an infinity or NaN.
  * Over FP8 and F16 pages f32 queries enter the products as two f16 terms, an element exact to 2^-22 of the largest of its row, and so
  * do the weights, whatever the type of q and o.
- * Scores (scale * q.k, and |q| * scale by itself) may have any size below 2^126, on either side of zero.  Elements of V in F32 pages must stay below 2^110: weights are kept up to 2^14 until the end. */
+ * Scores (scale * q.k, and |q| * scale by itself) may have any size below 2^126, on either side of zero.  Elements
+ * of V in F32 pages must stay below 2^110, under any number of keys. */
 typedef struct vfkv_paged_attn_params {
     uint32_t n_heads;
     uint32_t window;   /* 0: all keys up to the query's own */

@@ -80,6 +80,12 @@ hipError_t launch_paged_generic(const PagedAttnLaunch& L, hipStream_t stream);
 #ifdef __HIPCC__
 // Running maximum of a row that has seen no key yet: below every score.
 constexpr float kNoScore = -3.40282347e38f;
+// Weights are 2^(score - running maximum - ...): a maximum is raised when a score passes it by 2^kRaise, and a raised row's largest weight
+// is 2^kBias.  Over FP8 and F16 pages as large as f16 takes them (at most 2^14, smallest step 2^-30 of the largest).  Over F32 pages at
+// most 2^-6: 2^23 of them sum to 2^17, so elements of V up to 2^110 stay finite under any number of keys.
+constexpr float kRaise = 8.f;               // log2
+template <uint32_t DT>
+constexpr float kBias = DT == kF32 ? -14.f : 6.f;
 // A row is far out when its maximum (log2 units) leaves [-2^24, 2^24]: score * factor rounded once for the maximum and left exact
 // inside the multiply-add of a weight would differ by more than a unit of log2 there, and the weights leave their f16 range.
 __device__ __forceinline__ bool paged_far(float m) { return fabsf(m) > 16777216.f && m != kNoScore; }

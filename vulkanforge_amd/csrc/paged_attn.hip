@@ -60,7 +60,7 @@ __global__ __launch_bounds__(256) void paged_generic_kernel(PagedAttnLaunch a) {
             }
             const float mn = fmaxf(m, wave_max_all(x));
             const float corr = expf(m - mn);
-            const float pr = seen ? expf(x - mn) : 0.f;
+            const float pr = seen ? 0x1p-6f * expf(x - mn) : 0.f;            // (2^23 keys of 2^110 sum to a finite number)
             m = mn;
             l = l * corr + wave_sum_all(pr);
 #pragma unroll

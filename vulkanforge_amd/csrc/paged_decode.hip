@@ -25,8 +25,8 @@
 // 6.0 us for the join; one of 200 keys 6.5 us (the chain length -> page -> rows -> join of the wavefronts).  Rows of 512, 48 sequences of
 // up to 8 000 keys, 8 KV heads: FP8 310 us = 5.1 TB/s, F16 538 us = 5.8 TB/s.
 //
-//   - The running maximum is only raised when a score exceeds it by 2^8: weights are kept times 2^6 (at most 2^14 in f16, smallest
-//     step 2^-30 of the largest), and the accumulators are rescaled a few times per sequence instead of once per unit.
+//   - The running maximum is only raised when a score exceeds it by 2^8 (paged.h), so that the accumulators are rescaled a few times
+//     per sequence instead of once per unit.
 #include "device_utils.h"
 #include "paged.h"
 
@@ -36,7 +36,6 @@ namespace {
 
 constexpr int kDecWaves = 4;
 constexpr int kDecHeads = 8;               // query heads of a KV head per workgroup
-constexpr float kRaise = 8.f, kBias = 6.f;  // log2
 // What beginning a sequence costs a workgroup (queries, page numbers, the join of its wavefronts), in units: it stands in front of
 // the sequence's own units in the line.  Without it 124 sequences of 7 to 11 keys went to 16 workgroups of eight each.
 constexpr uint32_t kBegin = 2u * kDecWaves;
@@ -388,8 +387,8 @@ __global__ __launch_bounds__(256, D >= 256 ? 1 : 2) void paged_decode_kernel(Pag
             for (int t = 0; t < SUB; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) mx = fmaxf(mx, x[t][i]);
-            if (__any(mx * to_l2 - m > kRaise + kBias)) {
-                const float mn = fmaxf(m, max_over_groups(mx * to_l2) - kBias);
+            if (__any(mx * to_l2 - m > kRaise + kBias<DT>)) {
+                const float mn = fmaxf(m, max_over_groups(mx * to_l2) - kBias<DT>);
                 if (DT != kF32 && !(a.softcap > 0.f)) {
                     const bool now = __any(paged_far(mn));
                     if (now && !far) round_products();

@@ -15,7 +15,7 @@
 //   - f16 queries enter as they are, f32 queries as f16 value + remainder, and the weights as value + remainder for both: f32-level
 //     accuracy for one product more.  (Weights rounded to f16 are off by up to 2^-11 each, which large elements of V that cancel turn into
 //     ten steps of an f16 output.)  F32 caches use the f32 matrix instruction.
-//   - The running maximum is only raised when a score exceeds it by 2^8; weights are kept times 2^6 (see paged_decode.hip).
+//   - The running maximum is only raised when a score exceeds it by 2^8 (paged.h).
 // Measured (f16 product of 8 192 x 8 192 matrices in the library: 1 175 TFLOP/s): 8 192 tokens from position 0, FP8, f16 rows,
 // 32 / 8 / 128: 565-620 us by card = 890-974 TFLOP/s, the matrix units busy 0.41 and the vector units 0.39 of the time (LDS 0.31): the two
 // wavefronts of a SIMD meet at the tile's barrier, so half of what could overlap does.  512 tokens over 4 096 keys, f32 rows: 81-83 us =
@@ -34,8 +34,6 @@
 namespace vfkv {
 
 namespace {
-
-constexpr float kRaise = 8.f, kBias = 6.f;  // log2
 
 template <int DT, int D, int KT, int NW>
 struct PreShape {
@@ -430,8 +428,8 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
         for (int b = 0; b < NB; ++b)
 #pragma unroll
             for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[b][e]);
-        if (__any(mx * f - m > kRaise + kBias)) {
-            const float mn = fmaxf(m, max_over_halves(mx * f) - kBias);
+        if (__any(mx * f - m > kRaise + kBias<DT>)) {
+            const float mn = fmaxf(m, max_over_halves(mx * f) - kBias<DT>);
             if constexpr (!CAP) {
                 const uint32_t now = __builtin_amdgcn_readfirstlane(__any(paged_far(mn)) ? 1u : 0u);
                 if (__builtin_expect(now != 0u && far == 0u, 0)) round_products();
