@@ -101,7 +101,7 @@ __device__ __forceinline__ void block_prefix(const PagedAttnLaunch& a, uint32_t 
 }
 
 template <int DT, int D, bool IOF16, bool CAP, int KT, int CK, int NW, int MINW, int DS = 1>
-__global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnLaunch a, uint32_t n_split) {
+__global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnLaunch a, uint32_t n_split, uint32_t per_z) {
     using Z = PreShape<DT, D, KT, NW>;
     constexpr bool F32C = DT == kF32;
     constexpr bool QPAIR = !IOF16 && !F32C;                  // queries as value + remainder
@@ -120,7 +120,8 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n32 = lane & 31, hf = lane >> 5;
     // KV head fastest: consecutive workgroups go to different XCDs, so with eight heads each XCD keeps one head's keys in its L2
-    const uint32_t group = a.n_heads / a.c.n_kv_heads, block = blockIdx.x / a.c.n_kv_heads, kvh = blockIdx.x - block * a.c.n_kv_heads;
+    const uint32_t group = a.n_heads / a.c.n_kv_heads, block_x = blockIdx.x / a.c.n_kv_heads, kvh = blockIdx.x - block_x * a.c.n_kv_heads;
+    const uint32_t block = blockIdx.z * per_z + block_x;
     const uint32_t dr = a.c.head_dim;
     uint32_t* const pre = reinterpret_cast<uint32_t*>(lds);
     static_assert(2 * Z::BUF >= ((int)kPagedMaxSeqs + 1) * 4, "the prefix sums fit the tile buffers");
@@ -622,7 +623,9 @@ hipError_t launch_pre(const PagedAttnLaunch& L, hipStream_t stream) {
     const uint64_t with_rows = L.s.n_seqs < L.s.n_tokens ? L.s.n_seqs : L.s.n_tokens;
     uint64_t blocks = L.s.n_tokens * group / R + with_rows;
     if (blocks > L.s.n_tokens * group) blocks = L.s.n_tokens * group;
-    if (blocks * L.c.n_kv_heads * NW * 64u > 0xFFFFFFFFull) return hipErrorInvalidValue;   // (not with n_tokens * n_heads <= 2^30)
+    // a dimension of a launch holds fewer than 2^32 threads: the rest of the blocks along z (at most 2^30 workgroups in all)
+    const uint64_t room_x = 0xFFFFFFFFull / (NW * 64u) / L.c.n_kv_heads, per_z = blocks < room_x ? blocks : room_x;
+    if (per_z == 0u || (blocks + per_z - 1u) / per_z > 65535u) return hipErrorInvalidValue;   // (not with n_tokens * n_heads <= 2^30)
     // Split over the keys, as long as the card has room and a part has a tile: the tiles of a part against the join, which writes and
     // reads the parts once (about 4 TB/s and 3 us).  A tile takes about 2.2 us for f16 rows of 128 elements, 1.6 times that with
     // value + remainder, 6.8 us for 32 keys on the f32 instruction.  (FP8, 32 / 8 / 128, one part against two: 1 024 f16 tokens from
@@ -643,8 +646,8 @@ hipError_t launch_pre(const PagedAttnLaunch& L, hipStream_t stream) {
         const uint64_t ns = (tiles + i - 1u) / i * tile_ns + 3000u + rows * i * L.c.head_dim * 8u / 4000u;
         if (ns < best) { best = ns; n = i; }
     }
-    hipLaunchKernelGGL((paged_prefill_kernel<DT, D, IOF16, CAP, KT, CK, NW, MINW, DS>), dim3((uint32_t)(blocks * L.c.n_kv_heads), (uint32_t)n), dim3(NW * 64),
-                       LDS, stream, L, (uint32_t)n);
+    hipLaunchKernelGGL((paged_prefill_kernel<DT, D, IOF16, CAP, KT, CK, NW, MINW, DS>), dim3((uint32_t)(per_z * L.c.n_kv_heads), (uint32_t)n, (uint32_t)((blocks + per_z - 1u) / per_z)),
+                       dim3(NW * 64), LDS, stream, L, (uint32_t)n, (uint32_t)per_z);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || n == 1u) return e;
     return launch_paged_rows_merge(L, (uint32_t)n, stream);
