@@ -29,9 +29,11 @@ namespace vfkv {
 
 void clear_note() { g_note[0] = '\0'; }
 
-void note_generic(const char* who, uint32_t dtype, uint32_t head_dim) {
-    snprintf(g_note, sizeof(g_note), "%s: this shape (kv dtype %u, head_dim %u, or unaligned pointers / a layer slab of 2 GiB or more) "
-             "ran on the generic fallback kernel, 50-100x slower than the tiled kernels", who, dtype, head_dim);
+void set_note(const char* fmt, ...) {
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(g_note, sizeof(g_note), fmt, ap);
+    va_end(ap);
 }
 
 int fail(int status, const char* fmt, ...) {
@@ -52,7 +54,11 @@ namespace {
 
 using vfkv::fail;
 using vfkv::hip_fail;
-using vfkv::note_generic;
+
+void note_generic(const char* who, uint32_t dtype, uint32_t head_dim) {
+    vfkv::set_note("%s: this shape (kv dtype %u, head_dim %u, or unaligned pointers / a layer slab of 2 GiB or more) "
+                   "ran on the generic fallback kernel, 50-100x slower than the tiled kernels", who, dtype, head_dim);
+}
 
 #define VFKV_HIP(call)                                  \
     do {                                                \

@@ -18,6 +18,6 @@ namespace vfkv {
 int fail(int status, const char* fmt, ...) __attribute__((format(printf, 2, 3)));   // sets the thread's error text, returns status
 int hip_fail(hipError_t e, const char* what);
 void clear_note();
-void note_generic(const char* who, uint32_t dtype, uint32_t head_dim);
+void set_note(const char* fmt, ...) __attribute__((format(printf, 1, 2)));           // the thread's advisory (vfkv_last_note)
 
 }  // namespace vfkv

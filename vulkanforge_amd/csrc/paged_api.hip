@@ -469,6 +469,7 @@ static int paged_attention(vfkv_pages* c, uint32_t layer, const vfkv_seq_batch* 
     if ((rc = row_stride(p->q_stride, (uint64_t)p->n_heads * hd, who, "q", &L.q_stride)) != VFKV_OK) return rc;
     if ((rc = row_stride(p->o_stride, (uint64_t)p->n_heads * hd, who, "o", &L.o_stride)) != VFKV_OK) return rc;
     if (decode && b->q_offsets) return fail(VFKV_ERR_INVALID_ARG, "%s: one token per sequence (q_offsets must be NULL)", who);
+    vfkv::clear_note();
     if (nothing) return VFKV_OK;
     if (!q || !o) return fail(VFKV_ERR_INVALID_ARG, "%s: NULL buffer", who);
     if (q == o) return fail(VFKV_ERR_INVALID_ARG, "%s: o must not overlap q", who);
@@ -489,12 +490,15 @@ static int paged_attention(vfkv_pages* c, uint32_t layer, const vfkv_seq_batch* 
         // (rows of this call's head_dim: the workspace may have been made for wider ones)
         L.scratch_rows = (uint64_t)ws->n_heads * ws->max_tiles;
     }
-    vfkv::clear_note();
     const uint32_t per16 = p->io_dtype == VFKV_F32 ? 4u : 8u;
     const bool aligned = (((uintptr_t)q | (uintptr_t)o) & 15u) == 0u && L.q_stride % per16 == 0u && L.o_stride % per16 == 0u;
-    if (hd % 16u != 0u || hd > (c->cfg.dtype == VFKV_F32 ? 256u : 512u) || !aligned) {
+    const char* const why = hd % 16u != 0u ? "head_dim is not a multiple of 16"
+                            : c->cfg.dtype == VFKV_F32 && hd > 256u ? "rows of F32 pages are wider than 256 elements"
+                            : !aligned ? "q and o are not 16-byte aligned in every row" : nullptr;
+    if (why) {
         VFKV_HIP(vfkv::launch_paged_generic(L, S(stream)));
-        vfkv::note_generic(who, c->cfg.dtype, hd);
+        vfkv::set_note("%s: %s (kv dtype %u, head_dim %u): the call ran on the generic kernel, many times slower than the tiled kernels",
+                       who, why, c->cfg.dtype, hd);
         return VFKV_OK;
     }
     VFKV_HIP(decode ? vfkv::launch_paged_decode(L, S(stream)) : vfkv::launch_paged_prefill(L, S(stream)));
