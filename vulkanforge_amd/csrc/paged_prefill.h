@@ -444,25 +444,34 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
 #pragma unroll
                 for (int e = 0; e < 16; ++e) acc[n][e] *= corr;
         }
+        float sum = 0.f;                                     // of the chunk first: one by one, small weights would not reach a large l
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 sc[b][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][e], f, -m));
-                l += sc[b][e];
+                sum += sc[b][e];
             }
+        l += sum;
         if constexpr (F32C) {
+            // (the instruction adds two keys at a time: the chunk's sum first, for the same reason)
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
+            for (int n = 0; n < DT32; ++n) {
+                float16_t part;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const uint8_t* const vrow = vl + (32 * b + 8 * (e / 4) + 4 * hf + e % 4) * Z::VPITCH + n32 * 4;
+                for (int e = 0; e < 16; ++e) part[e] = 0.f;
 #pragma unroll
-                    for (int n = 0; n < DT32; ++n) {
-                        const float v = *reinterpret_cast<const float*>(vrow + 128 * n);
-                        acc[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, sc[b][e], acc[n], 0, 0, 0);
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float v = *reinterpret_cast<const float*>(vl + (32 * b + 8 * (e / 4) + 4 * hf + e % 4) * Z::VPITCH + n32 * 4 + 128 * n);
+                        part = __builtin_amdgcn_mfma_f32_32x32x2f32(v, sc[b][e], part, 0, 0, 0);
                     }
-                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[n][e] += part[e];
+                // (the next columns' loads, moved up to here, spill: 512 x 4 608, rows of 128, 356 us against 328)
+                __builtin_amdgcn_sched_barrier(0);
+            }
         } else {
             // lane's place in the transposing read: row 4 hf + (lane % 16) / 4 of eight-row steps, column group of its sixteen lanes
             const uint8_t* const vlane = vl + (4 * hf + (lane & 15) / 4) * Z::VPITCH + (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
