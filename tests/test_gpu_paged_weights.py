@@ -39,3 +39,22 @@ def test_f16_rows_round_only_at_the_output(dtype, d, hq, hkv, peaked, window, si
         torch.cuda.synchronize()
         ref, bound = exact(pool, q, lens, window, sink, softcap)
         assert_near(o, ref, bound, torch.float16, "decode" if decode else "prefill")
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, F8])
+@pytest.mark.parametrize("d, hq, hkv", [(64, 4, 1), (128, 8, 2), (256, 4, 2), (512, 4, 2), (40, 2, 1)])
+@pytest.mark.parametrize("window, sink", [(0, 0), (3000, 70)])
+def test_f16_rows_over_long_contexts(dtype, d, hq, hkv, window, sink):
+    """Outputs of a few hundredths, where a key lost or counted twice is more than the bound of an element."""
+    kv, q_len = [5000, 2049, 1], [7, 40, 1]
+    pool = Pool(dtype, hkv, d, 64, kv, seed=d)
+    g = torch.Generator().manual_seed(d)
+    for decode in (False, True):
+        lens = [1] * 3 if decode else q_len
+        q = torch.randn((sum(lens), hq, d), generator=g).half().to(DEV)
+        o = torch.full_like(q, float("nan"))
+        fwd = vf.PagedForward(pool.cache, hq)
+        (fwd.decode_attention if decode else fwd.prefill_attention)(0, pool.batch(None if decode else lens), q, o, window=window, n_sink=sink)
+        torch.cuda.synchronize()
+        ref, bound = exact(pool, q, lens, window, sink)
+        assert_near(o, ref, bound, torch.float16, "decode" if decode else "prefill")
