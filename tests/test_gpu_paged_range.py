@@ -93,3 +93,24 @@ def test_only_keys_far_below_zero(decode, d):
             for s, kv in enumerate(pool.kv):
                 mean = pool.rows(pool.v, s).mean(0).expand(2, d)
                 assert (o[s].cpu().double() - mean).abs().max() <= 4.0 * (kv / 16 + 72) * 2.0 ** -24 * (1 + math.log2(kv)), (dtype, size)
+
+
+@pytest.mark.parametrize("dtype", [F16, F8])
+@pytest.mark.parametrize("decode", [True, False])
+def test_rows_far_out_leave_the_ordinary_ones_alone(dtype, decode):
+    """Every other head with scores beyond 2^30: the heads between them give what they give without, to the steps of their weights (the
+    running maximum is raised for all rows of a wavefront at once): two weights of 22 bits times elements below 5 that sum to 1."""
+    pool = Pool(dtype, 1, 128, 32, [500, 90])
+    lens = [1, 1] if decode else [60, 9]
+    q = torch.randn((sum(lens), 4, 128), generator=torch.Generator().manual_seed(2)).to(DEV)
+    outs = []
+    for by in (1.0, 2.0 ** 31):
+        q2 = q.clone()
+        q2[:, 1::2] *= by
+        o = torch.full_like(q, float("nan"))
+        fwd = vf.PagedForward(pool.cache, 4)
+        (fwd.decode_attention if decode else fwd.prefill_attention)(0, pool.batch(None if decode else lens), q2, o)
+        torch.cuda.synchronize()
+        assert bool(o.isfinite().all())
+        outs.append(o[:, ::2])
+    assert (outs[0] - outs[1]).abs().max() <= 2 * 5 * 2.0 ** -22

@@ -271,7 +271,7 @@ __global__ __launch_bounds__(256, D >= 256 ? 1 : 2) void paged_decode_kernel(Pag
 #pragma unroll
         for (int n = 0; n < Z::NT; ++n) acc[n] = float4_t{0.f, 0.f, 0.f, 0.f};
         float m = kNoScore, l = 0.f;                                     // l: this lane's keys only, summed at the end
-        bool far = false;                                                // some row is far out: products are rounded before they are compared
+        bool far = false;                                                // some head is far out: its products are rounded before they are compared
 
         auto unit_key = [&](uint32_t u) { return (u < Q.sink_units ? u : Q.first + u - Q.sink_units) * (uint32_t)Z::UK; };
         auto get_pages = [&](uint32_t u) {
@@ -362,14 +362,17 @@ __global__ __launch_bounds__(256, D >= 256 ? 1 : 2) void paged_decode_kernel(Pag
 #pragma unroll
                     for (int i = 0; i < 4; ++i) x[t][i] = paged_softcap_l2(x[t][i] * fac, cap_l2, inv_cap_l2);
             }
-            auto round_products = [&] {
-                to_l2 = 1.0f;
+            bool rounded = false;
+            auto round_products = [&](bool mine) {                       // of this lane's head; the others keep theirs
+                const float by = mine ? fac : 1.0f;
+                to_l2 = mine ? 1.0f : to_l2;
+                rounded = rounded || mine;
 #pragma unroll
                 for (int t = 0; t < SUB; ++t)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) x[t][i] *= fac;
+                    for (int i = 0; i < 4; ++i) x[t][i] *= by;
             };
-            if (DT != kF32 && far) round_products();                     // (F32: fac is 1; far is never set with a soft-cap)
+            if (DT != kF32 && far) round_products(paged_far(m));         // (F32: fac is 1; far is never set with a soft-cap)
             if (!full) {
 #pragma unroll
                 for (int t = 0; t < SUB; ++t)
@@ -390,9 +393,8 @@ __global__ __launch_bounds__(256, D >= 256 ? 1 : 2) void paged_decode_kernel(Pag
             if (__any(mx * to_l2 - m > kRaise + kBias<DT>)) {
                 const float mn = fmaxf(m, max_over_groups(mx * to_l2) - kBias<DT>);
                 if (DT != kF32 && !(a.softcap > 0.f)) {
-                    const bool now = __any(paged_far(mn));
-                    if (now && !far) round_products();
-                    far = now;
+                    far = __any(paged_far(mn));
+                    if (far) round_products(paged_far(mn) && !rounded);
                 }
                 const float corr = __builtin_amdgcn_exp2f(m - mn);
                 m = mn;

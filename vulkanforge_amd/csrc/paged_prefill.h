@@ -258,7 +258,7 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
 
     float16_t acc[DT32];
     float m = kNoScore, l = 0.f;                             // l: this lane's keys only, summed at the end
-    uint32_t far = 0u;                                       // some row is far out: products are rounded before they are compared
+    uint32_t far = 0u;                                       // some row is far out: its products are rounded before they are compared
 #pragma unroll
     for (int n = 0; n < DT32; ++n)
 #pragma unroll
@@ -395,14 +395,17 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
                 for (int e = 0; e < 16; ++e) sc[b][e] = paged_softcap_l2(sc[b][e] * qmul, cap_l2, inv_cap_l2);
         }
         float f = fac;
-        auto round_products = [&] {
-            f = 1.0f;
+        bool rounded = false;
+        auto round_products = [&](bool mine) {               // of this lane's row; the others keep theirs
+            const float by = mine ? fac : 1.0f;
+            f = mine ? 1.0f : f;
+            rounded = rounded || mine;
 #pragma unroll
             for (int b = 0; b < NB; ++b)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) sc[b][e] *= fac;
+                for (int e = 0; e < 16; ++e) sc[b][e] *= by;
         };
-        if (!CAP && __builtin_expect(far != 0u, 0)) round_products();
+        if (!CAP && __builtin_expect(far != 0u, 0)) round_products(paged_far(m));
         if (masked) {
             // key in [lo, pos] as one unsigned comparison against their number; a key among the first tokens as another
             auto hide = [&](auto firsts) {
@@ -432,9 +435,8 @@ __global__ __launch_bounds__(NW * 64, MINW) void paged_prefill_kernel(PagedAttnL
         if (__any(mx * f - m > kRaise + kBias<DT>)) {
             const float mn = fmaxf(m, max_over_halves(mx * f) - kBias<DT>);
             if constexpr (!CAP) {
-                const uint32_t now = __builtin_amdgcn_readfirstlane(__any(paged_far(mn)) ? 1u : 0u);
-                if (__builtin_expect(now != 0u && far == 0u, 0)) round_products();
-                far = now;
+                far = __builtin_amdgcn_readfirstlane(__any(paged_far(mn)) ? 1u : 0u);
+                if (__builtin_expect(far != 0u, 0)) round_products(paged_far(mn) && !rounded);
             }
             const float corr = __builtin_amdgcn_exp2f(m - mn);
             m = mn;
