@@ -23,7 +23,8 @@
 // Measured, one layer (copy rate of the card: 5.2 TB/s): 48 sequences of 17-8 193 keys, FP8, 32 / 8 / 128: 80.6 us = 4.8 TB/s; 12 windows
 // of 4 096 keys, F16, 16 / 8 / 256, soft-capped: 77.1 us = 5.0 TB/s; one sequence of 65 536 keys: 25.8 us for the worker (5.2 TB/s) and
 // 6.0 us for the join; one of 200 keys 6.5 us (the chain length -> page -> rows -> join of the wavefronts).  Rows of 512, 48 sequences of
-// up to 8 000 keys, 8 KV heads: FP8 310 us = 5.1 TB/s, F16 538 us = 5.8 TB/s.
+// up to 8 000 keys, 8 KV heads: FP8 310 us = 5.1 TB/s, F16 538 us = 5.8 TB/s.  F32 pages, the first batch: 291 us = 5.3 TB/s, with 19
+// registers spilled (6 at rows of 256).
 //
 //   - The running maximum is only raised when a score exceeds it by 2^8 (paged.h), so that the accumulators are rescaled a few times
 //     per sequence instead of once per unit.
@@ -35,7 +36,9 @@ namespace vfkv {
 namespace {
 
 constexpr int kDecWaves = 4;
-constexpr int kDecHeads = 8;               // query heads of a KV head per workgroup
+// Query heads of a KV head per workgroup: a larger group is cut into slices of eight, each of which reads the keys again (48 sequences of
+// 17-8 193 keys, FP8, 64 / 4 heads 72.9 us, 32 / 4 50.5; 12 / 1 29.0, 8 / 1 23.5).
+constexpr int kDecHeads = 8;
 // What beginning a sequence costs a workgroup (queries, page numbers, the join of its wavefronts), in units: it stands in front of
 // the sequence's own units in the line.  Without it 124 sequences of 7 to 11 keys went to 16 workgroups of eight each.
 constexpr uint32_t kBegin = 2u * kDecWaves;

@@ -17,12 +17,13 @@
 //     ten steps of an f16 output.)  F32 caches use the f32 matrix instruction.
 //   - The running maximum is only raised when a score exceeds it by 2^8 (paged.h).
 // Measured (f16 product of 8 192 x 8 192 matrices in the library: 1 175 TFLOP/s): 8 192 tokens from position 0, FP8, f16 rows,
-// 32 / 8 / 128: 565-620 us by card = 890-974 TFLOP/s, the matrix units busy 0.41 and the vector units 0.39 of the time (LDS 0.31): the two
-// wavefronts of a SIMD meet at the tile's barrier, so half of what could overlap does.  512 tokens over 4 096 keys, f32 rows: 81-83 us =
-// 450 TFLOP/s of useful work, 900 with the remainder products.  Windows of 1 024 keys: 560-575 TFLOP/s (18 tiles per block do not
-// hide a block's beginning and end).  Tried and not kept: two row blocks per wavefront (one wavefront per SIMD, 461 TFLOP/s: the
-// accumulators no longer fit the registers the matrix instructions take), tiles of 128 keys, raised wave priority around the
-// products, the first tile requested before the queries (all within 3 %).
+// 32 / 8 / 128: 750-785 us by card = 700-735 TFLOP/s of useful work, 1 050-1 100 with the remainder product, the matrix units busy 0.50 and
+// the vector units 0.45 of the time (LDS 0.25): the two wavefronts of a SIMD meet at the tile's barrier, so half of what could overlap
+// does.  512 tokens over 4 096 keys, f32 rows: 83 us = 440 TFLOP/s of useful work, 880 with the remainder products.  Windows of 1 024
+// keys, f16 rows: 507 (F16 pages) and 555 (FP8) TFLOP/s of useful work (18 tiles per block do not hide a block's beginning and end).  F32
+// pages, 512 tokens over 4 096 keys: 328 us = 111 TFLOP/s of the f32 instruction's 154 in the library.  Tried and not kept: two row
+// blocks per wavefront (one wavefront per SIMD, half the rate: the accumulators no longer fit the registers the matrix instructions
+// take), tiles of 128 keys, raised wave priority around the products, the first tile requested before the queries (all within 3 %).
 //
 //   - Few rows over many keys: the tiles are cut into n_split parts over more workgroups and joined by paged_rows_merge_kernel.
 #pragma once
@@ -638,9 +639,10 @@ hipError_t launch_pre(const PagedAttnLaunch& L, hipStream_t stream) {
     const uint64_t room_x = 0xFFFFFFFFull / (NW * 64u) / L.c.n_kv_heads, per_z = blocks < room_x ? blocks : room_x;
     if (per_z == 0u || (blocks + per_z - 1u) / per_z > 65535u) return hipErrorInvalidValue;   // (not with n_tokens * n_heads <= 2^30)
     // Split over the keys, as long as the card has room and a part has a tile: the tiles of a part against the join, which writes and
-    // reads the parts once (about 4 TB/s and 3 us).  A tile takes about 2.2 us for f16 rows of 128 elements, 1.6 times that with
-    // value + remainder, 6.8 us for 32 keys on the f32 instruction.  (FP8, 32 / 8 / 128, one part against two: 1 024 f16 tokens from
-    // position 0 33.6 / 39.5 us, over 5 000 keys 162 / 104 us; 7 tokens over 1 000 keys, F16 heads of 64, 4 / 16 parts 17.6 / 12.6 us.)
+    // reads the parts once (about 4 TB/s and 3 us).  A tile takes 1.8 us (four wavefronts) to 2.5 us (eight) for f16 rows of 128
+    // elements, 1.6 times that for f32 rows, 6.8 us for 32 keys on the f32 instruction.  (FP8, 32 / 8 / 128, one part against two: 1 024
+    // f16 tokens from position 0 38.1 / 45.9 us, over 5 000 keys 237 / 150 us; 7 tokens over 1 000 keys, F16 heads of 64, 4 / 16 parts
+    // 15.0 / 11.3 us.)
     constexpr uint64_t tile_ns = (DT == kF32 ? 6800u * KT / 32u : (IOF16 ? 2200u : 3500u) * KT / 64u) * (D / DS) / 128u;
     const uint64_t likely = (L.s.n_tokens * group + R - 1u) / R * L.c.n_kv_heads;
     // (unlike blocks: twice the workgroups that fit, so that the last ones are short; F16 rows of 256, 2 048 tokens 129 -> 105 us)
@@ -675,21 +677,22 @@ hipError_t launch_dim(const PagedAttnLaunch& L, hipStream_t stream) {
         // Workgroups of eight wavefronts share a staged tile among twice the rows, but a card that they fill only once waits for the
         // block with the most keys: they are taken for chunks that fill blocks of 256 rows, with two rounds of blocks or with a
         // context that makes the blocks alike.  (FP8 / f16 rows of 128, eight / four wavefronts: 4 096 tokens from position 0
-        // 160 / 172 us, 2 048 76 / 65 us, 1 024 tokens over 5 000 keys 102 / 110 us; F16 rows of 256: 8 192 tokens 753 / 1 012 us,
-        // 4 096 327 / 271 us, 2 048 over 6 000 keys 301 / 356 us.)
+        // 203 / 222 us, 2 048 90 / 76 us, 1 024 tokens over 5 000 keys 150 / 159 us; F16 rows of 256: 8 192 tokens 953 / 1 204 us,
+        // 4 096 424 / 323 us, 2 048 over 6 000 keys 476 / 571 us.  At 256 elements the eight spill 20 (FP8) or 34 (F16) registers, counted
+        // in these figures.)
         const uint64_t rows = (uint64_t)L.s.n_tokens * (L.n_heads / L.c.n_kv_heads);
         // Short windows, rows of up to 128: two workgroups of four on a CU, one of which begins or ends a block while the other
-        // computes.  (Eight / four: FP8 / f16 rows, 2 x 4 096 tokens, window 128 92.5 / 78.5 us, 4 096, window 512 71.7 / 66.2, 8 192, window 1 024 202 / 187,
-        // 4 096 over 16 384, window 4 096 304 / 317; F16 pages 97.8 / 88.5, 74.3 / 72.9, 211 / 209, 320 / 352; FP8 / f32 rows 109 / 99,
-        // 90 / 92, 289 / 280, 479 / 500.)
+        // computes.  (Eight / four: FP8 / f16 rows, 2 x 4 096 tokens, window 128 102 / 86 us, 4 096, window 512 84 / 78, 8 192, window 1 024 250 / 232,
+        // 4 096 over 16 384, window 4 096 392 / 403; F16 pages 107 / 97, 86.3 / 85.7, 259 / 255, 411 / 442; FP8 / f32 rows 109 / 99,
+        // 90 / 92, 289 / 280, 479 / 500.  Between 384 and 1 536 the two are within 2 % over F16 pages and within 3 % for f32 rows.)
         const bool brief = d <= 128u && L.window != 0u && (uint64_t)L.window + L.n_sink <= (DT == kF8 && IOF16 ? 1536u : 384u);
         const bool many = !brief && rows >= 256ull * L.s.n_seqs && (blocks_alike(L) || rows / 256u * L.c.n_kv_heads >= 512u);
         constexpr int CK = IOF16 ? 64 : 32, KT = 64;
         if (d <= 64u) return many ? launch_pre<DT, 64, IOF16, CAP, 64, 64, 8, 2>(L, stream) : launch_pre<DT, 64, IOF16, CAP, 64, 64, 4, 2>(L, stream);
         if (d <= 128u) return many ? launch_pre<DT, 128, IOF16, CAP, KT, CK, 8, 2>(L, stream) : launch_pre<DT, 128, IOF16, CAP, KT, CK, 4, 2>(L, stream);
         // rows of 512: two wavefronts per block of 32 rows, each half of the columns of both products, their scores added through LDS
-        // (16 / 2 heads, FP8, f16 rows: 512 tokens over 4 096 keys 215 us = 340 TFLOP/s, 4 096 from position 0 688 us = 400; one
-        // workgroup per CU, two barriers per tile; the generic kernel: 43 ms)
+        // (16 / 2 heads, FP8, f16 rows: 512 tokens over 4 096 keys 219 us = 333 TFLOP/s of useful work, 4 096 from position 0 755 us = 364;
+        // one workgroup per CU, two barriers per tile; the generic kernel: 43 ms)
         if (d > 256u) return launch_pre<DT, 512, IOF16, CAP, 32, 32, 4, 1, 2>(L, stream);
         if constexpr (IOF16)                                     // (value + remainder of 256 elements do not fit 256 registers)
             if (many) return launch_pre<DT, 256, IOF16, CAP, 32, 32, 8, 2>(L, stream);
